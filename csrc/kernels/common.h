@@ -10,7 +10,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // Activation codes shared with the Python side (ops/_native.py).
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SIGMOID = 2,
-       ACT_TANH = 3 };   // tanh: stand-alone activation / activation-gradient kernels only (the GEMM epilogues fuse relu and sigmoid)
+       ACT_TANH = 3,     // tanh: stand-alone activation / activation-gradient kernels only (the GEMM epilogues fuse relu and sigmoid)
+       ACT_SILU = 4 };   // silu (u sigmoid(u)): group normalisation only
 
 #define DTF_CHECK_LAUNCH()                               \
     do {                                                 \

@@ -7,6 +7,7 @@ the CPU reference implementations in this package only run for CPU tensors.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 from pathlib import Path
@@ -16,6 +17,7 @@ import torch
 LIB_DIR = Path(__file__).resolve().parent.parent / "_lib"
 
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
+ACT_SILU = 4        # u * sigmoid(u): group normalisation only
 ACT_CODES = {None: ACT_NONE, "linear": ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "sigmoid": ACT_SIGMOID,
              "tanh": ACT_TANH}
 
@@ -84,6 +86,13 @@ def kernels():
         "dtf_batchnorm_fwd": [c_p, c_p, c_ll, c_i, c_p, c_p, c_p, c_p, c_f, c_f, c_i, c_p, c_p, c_p, c_p],
         "dtf_batchnorm_bwd": [c_p, c_p, c_p, c_ll, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p],
         "dtf_softmax_rows": [c_p, c_p, c_i, c_i, c_p],
+        "dtf_global_norm_partials": [],
+        "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, c_f, c_p, c_p, c_p],
+        "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p],
+        "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
+        "dtf_linear_xent_fwd": [c_p, c_p, c_p, c_p, c_ll, c_ll, c_ll, c_i, c_i, c_ll, c_p, c_p, c_p, c_p, c_p, c_p],
+        "dtf_linear_xent_bwd": [c_p, c_p, c_p, c_p, c_ll, c_ll, c_ll, c_i, c_i, c_ll, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_p,
+                                c_p, c_p, c_p],
         "dtf_im2col": [c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_col2im": [c_p, c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_avgpool_fwd": [c_p, c_p] + [c_i] * 12 + [c_p],
@@ -116,6 +125,10 @@ def kernels():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
             fn.restype = c_i
+    for name, argtypes in {"dtf_groupnorm_workspace_floats": [c_ll, c_ll, c_i, c_i],
+                           "dtf_linear_xent_fwd_workspace_bytes": [c_ll, c_ll, c_ll, c_i, c_i],
+                           "dtf_linear_xent_bwd_workspace_bytes": [c_ll, c_ll, c_ll, c_i, c_i]}.items():
+        declare(lib, name, argtypes, c_ll)
     if hasattr(lib, "dtf_batchnorm_workspace_floats"):
         lib.dtf_batchnorm_workspace_floats.argtypes = [c_ll, c_i]
         lib.dtf_batchnorm_workspace_floats.restype = c_ll
@@ -151,6 +164,14 @@ def stream_ptr() -> int:
     for it: the binding's own entry point is used, `torch.cuda.current_stream()` builds a Python stream object and
     resolves the device through several layers, ~3 us per call."""
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def device_guard(t):
+    """Context in which ``t``'s device is the current one (and ``stream_ptr`` its current stream)."""
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == t.device.index else torch.cuda.device(t.device)
 
 
 def ptr(t) -> int:

@@ -134,6 +134,49 @@ def softmax_cross_entropy(logits, labels):
     return _SoftmaxXentFn.apply(logits, labels)
 
 
+class _LinearXentFn(torch.autograd.Function):
+    """Softmax cross-entropy of ``x @ w + b`` without the logits in memory; the backward pass is computed when it is asked
+    for, from the rows' logsumexp."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, labels, ignore_index, reduction, bf16):
+        loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16)
+        ctx.save_for_backward(x, w, b, labels, *state)
+        ctx.cfg = (ignore_index, reduction, bf16)
+        if reduction == "none":
+            return loss
+        return state.totals[2 if reduction == "mean" else 0].clone()
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, w, b, labels = ctx.saved_tensors[:4]
+        state = F.LinearXentState(*ctx.saved_tensors[4:])
+        ignore_index, reduction, bf16 = ctx.cfg
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty_like(w) if need[1] else None
+        db = torch.empty_like(b) if b is not None and need[2] else None
+        F.linear_xent_backward(x, w, b, labels, state, _c(dloss), reduction == "mean", ignore_index, bf16, dx, dw, db)
+        return dx, dw, db, None, None, None, None
+
+
+def linear_softmax_cross_entropy(x, w, labels, b=None, ignore_index: int = -1, reduction: str = "mean", bf16: bool = False):
+    """Softmax cross-entropy of a linear head over a large vocabulary, ``softmax_cross_entropy(dense(x, w, b), labels)``
+    without the logits in memory: ``x`` [..., K], ``w`` [K, V], ``b`` [V] or None (all float32 or all bfloat16), int64
+    ``labels`` [...].  The loss is float32: the mean over the rows whose label is not ``ignore_index`` (0 when there are
+    none), their ``"sum"``, or with ``reduction="none"`` every row's own in the shape of ``labels`` (0 in ignored rows).
+    ``bf16=True`` rounds float32 operands to bfloat16 for the products."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
+    if tuple(labels.shape) != tuple(x.shape[:-1]):
+        raise ValueError("labels %s do not fit x %s" % (tuple(labels.shape), tuple(x.shape)))
+    c = lambda t: None if t is None else t.contiguous()
+    loss = _LinearXentFn.apply(c(x.reshape(-1, x.shape[-1])), c(w), c(b), c(labels.reshape(-1).to(torch.int64)),
+                               int(ignore_index), reduction, bool(bf16))
+    return loss.reshape(labels.shape) if reduction == "none" else loss
+
+
 class _MseFn(torch.autograd.Function):
     """Keras ``mean_squared_error`` averaged over the batch: mean over all elements of ``(p - y)^2``."""
 
@@ -315,6 +358,42 @@ def batch_norm(x, gamma, beta, moving_mean, moving_var, momentum: float = 0.99, 
     return _BatchNormFn.apply(x, gamma, beta, moving_mean, moving_var, float(momentum), float(eps), bool(training))
 
 
+class _GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, groups, eps, act):
+        gamma, beta = _c(gamma), _c(beta)
+        y, stats = F.groupnorm_forward(x, gamma, beta, groups, eps, act)
+        ctx.save_for_backward(x, gamma, beta, stats)
+        ctx.cfg = (groups, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, stats = ctx.saved_tensors
+        groups, act = ctx.cfg
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dgamma = torch.empty_like(gamma) if gamma is not None and need[1] else None
+        dbeta = torch.empty_like(beta) if beta is not None and need[2] else None
+        F.groupnorm_backward(x, dy.contiguous(), gamma, beta, groups, stats, act, dgamma, dbeta, dx)
+        return dx, dgamma, dbeta, None, None, None
+
+
+def group_norm(x, gamma, beta, groups: int, eps: float = 1e-3, activation=None):
+    """Differentiable ``activation(group_normalisation(x))`` over the last axis of a channels-last ``x`` [B, ..., C] (float32,
+    bfloat16 or float16): the channels of every sample in ``groups`` groups, each over all its positions.  ``gamma`` /
+    ``beta`` [C] may be None; ``activation``: None, 'relu', 'sigmoid', 'tanh' or 'silu'."""
+    return _GroupNormFn.apply(x.contiguous(), gamma, beta, int(groups), float(eps), F.groupnorm_activation(activation))
+
+
+def clip_grad_norm(parameters, max_norm: float):
+    """Clips the gradients of ``parameters`` in place by their global norm and returns the norm (a float32 scalar tensor) that
+    they had before; call it between ``backward()`` and the optimizer's ``step()``."""
+    grads = [p.grad for p in parameters if p.grad is not None]
+    return F.clip_by_global_norm(grads, max_norm, out=grads)[1]
+
+
 # ----------------------------------------------------------------------------------------------- torch.nn modules
 class Dense(torch.nn.Module):
     """``torch.nn.Module`` whose forward and backward are the fused HIP dense kernels (Glorot-uniform kernel
@@ -372,3 +451,35 @@ class BatchNormalization(torch.nn.Module):
     def forward(self, x):
         return batch_norm(x, self.gamma, self.beta, self.moving_mean, self.moving_variance, self.momentum, self.epsilon,
                           self.training)
+
+
+class GroupNormalization(torch.nn.Module):
+    """Keras-style group normalisation of channels-last tensors with an activation, on the HIP kernels."""
+
+    def __init__(self, channels: int, groups: int = 32, epsilon: float = 1e-3, center: bool = True, scale: bool = True,
+                 activation: Optional[str] = None):
+        super().__init__()
+        if channels % groups:
+            raise ValueError("%d channels do not divide into %d groups" % (channels, groups))
+        self.gamma = torch.nn.Parameter(torch.ones(channels)) if scale else None
+        self.beta = torch.nn.Parameter(torch.zeros(channels)) if center else None
+        self.groups, self.epsilon, self.activation = int(groups), float(epsilon), activation
+        F.groupnorm_activation(activation)
+
+    def forward(self, x):
+        return group_norm(x, self.gamma, self.beta, self.groups, self.epsilon, self.activation)
+
+
+class SoftmaxCrossEntropyHead(torch.nn.Module):
+    """A linear layer over a large vocabulary together with its softmax cross-entropy: ``forward(x, labels)`` is the loss, and
+    the logits are never in memory (``kernel`` [in, classes], Glorot-uniform; zero bias)."""
+
+    def __init__(self, in_features: int, classes: int, use_bias: bool = True, ignore_index: int = -1, reduction: str = "mean"):
+        super().__init__()
+        limit = math.sqrt(6.0 / (in_features + classes))
+        self.kernel = torch.nn.Parameter((torch.rand(in_features, classes) * 2.0 - 1.0) * limit)
+        self.bias = torch.nn.Parameter(torch.zeros(classes)) if use_bias else None
+        self.ignore_index, self.reduction = int(ignore_index), reduction
+
+    def forward(self, x, labels):
+        return linear_softmax_cross_entropy(x, self.kernel, labels, self.bias, self.ignore_index, self.reduction)

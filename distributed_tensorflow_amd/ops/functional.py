@@ -13,10 +13,14 @@ and the Adam apply).
 """
 from __future__ import annotations
 
+import collections
+import ctypes
+import math
+
 import torch
 
 from . import _native as nv
-from ._native import ACT_CODES, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH  # noqa: F401
+from ._native import ACT_CODES, ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_SILU, ACT_TANH  # noqa: F401
 
 _M32 = 0xFFFFFFFF
 
@@ -328,6 +332,132 @@ def batchnorm_backward(x, dy, gamma, save_mean, save_inv_std, dgamma=None, dbeta
     return dx
 
 
+# --------------------------------------------------------------------------- group normalisation
+GROUPNORM_ACTIVATIONS = dict(ACT_CODES, silu=ACT_SILU, swish=ACT_SILU)
+_GROUPNORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def groupnorm_activation(name) -> int:
+    if name not in GROUPNORM_ACTIVATIONS:
+        raise ValueError("unsupported activation %r (have: relu, sigmoid, tanh, silu, linear)" % (name,))
+    return GROUPNORM_ACTIVATIONS[name]
+
+
+def _groupnorm_sizes(x, groups, gamma, beta, *others):
+    """``(B, S, C)`` of a channels-last ``x`` [B, ..., C] after the checks that both directions share."""
+    if x.dim() < 2:
+        raise ValueError("group normalisation takes [batch, ..., channels], got shape %s" % (tuple(x.shape),))
+    if x.dtype not in _GROUPNORM_TYPES:
+        raise ValueError("group normalisation takes float32, bfloat16 or float16, got %s" % x.dtype)
+    C = int(x.shape[-1])
+    if groups < 1 or C < 1 or C % groups:
+        raise ValueError("%d channels do not divide into %d groups" % (C, groups))
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()
+                              or t.device != x.device):
+            raise ValueError("%s must be a contiguous float32 tensor of %d channels on %s" % (name, C, x.device))
+    for t in (x,) + others:
+        if t is not None and (t.dtype != x.dtype or t.shape != x.shape or not t.is_contiguous() or t.device != x.device):
+            raise ValueError("group normalisation takes contiguous tensors of one type, shape and device")
+    return int(x.shape[0]), math.prod(x.shape[1:-1]), C
+
+
+def _groupnorm_act(u, act):
+    return u * torch.sigmoid(u) if act == ACT_SILU else _apply_act(u, act)
+
+
+def groupnorm_forward(x, gamma, beta, groups, eps=1e-3, act=ACT_NONE, out=None, stats=None):
+    """``act(gamma xhat + beta)`` of a channels-last ``x`` [B, ..., C]: every sample's channels are normalised in ``groups``
+    groups of C / groups neighbours over all positions (biased variance).  ``gamma`` / ``beta`` [C] float32 may be None.
+    Returns ``(y, stats)``; ``stats`` [3, B, groups] float32 (mean, what the mean's rounding to float32 left, 1 / standard
+    deviation) is what ``groupnorm_backward`` needs."""
+    B, S, C = _groupnorm_sizes(x, groups, gamma, beta, out)
+    if out is None:
+        out = torch.empty_like(x)
+    if stats is None:
+        stats = torch.empty((3, B, groups), dtype=torch.float32, device=x.device)
+    elif tuple(stats.shape) != (3, B, groups) or stats.dtype != torch.float32 or not stats.is_contiguous() \
+            or stats.device != x.device:
+        raise ValueError("stats must be a contiguous float32 tensor of shape %s on %s" % ((3, B, groups), x.device))
+    if x.numel() == 0:
+        stats.zero_()
+        return out, stats
+    if x.is_cuda:
+        with nv.device_guard(x):
+            rc = nv.kernels().dtf_groupnorm_fwd(nv.ptr(x), nv.ptr(out), B, S, C, groups, _GROUPNORM_TYPES[x.dtype], nv.ptr(gamma),
+                                                nv.ptr(beta), float(eps), int(act), nv.ptr(stats), nv.stream_ptr())
+        nv.check(rc, "dtf_groupnorm_fwd")
+        return out, stats
+    v = x.to(torch.float64).view(B, S, groups, C // groups)
+    mean = v.mean(dim=(1, 3))
+    var = v.var(dim=(1, 3), unbiased=False)
+    stats[0].copy_(mean)
+    stats[1].copy_(mean - stats[0].double())
+    stats[2].copy_(1.0 / torch.sqrt(var + eps))
+    u = _groupnorm_xhat(x, groups, stats)
+    u = u if gamma is None else u * gamma
+    out.copy_(_groupnorm_act(u if beta is None else u + beta, act))
+    return out, stats
+
+
+def _groupnorm_xhat(x, groups, stats):
+    B, C = x.shape[0], x.shape[-1]
+    s = stats.view(3, B, 1, groups, 1)
+    return (((x.float().view(B, -1, groups, C // groups) - s[0]) - s[1]) * s[2]).view(x.shape)
+
+
+def groupnorm_backward(x, dy, gamma, beta, groups, stats, act=ACT_NONE, dgamma=None, dbeta=None, dx=None):
+    """Gradient of ``groupnorm_forward`` into ``dx`` (like x) and ``dgamma`` / ``dbeta`` [C] float32; each may be None."""
+    B, S, C = _groupnorm_sizes(x, groups, gamma, beta, dy, dx)
+    if tuple(stats.shape) != (3, B, groups) or stats.dtype != torch.float32 or not stats.is_contiguous() \
+            or stats.device != x.device:
+        raise ValueError("stats must be what groupnorm_forward returned")
+    for name, t in (("dgamma", dgamma), ("dbeta", dbeta)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()
+                              or t.device != x.device):
+            raise ValueError("%s must be a contiguous float32 tensor of %d channels on %s" % (name, C, x.device))
+    if x.numel() == 0:
+        for t in (dgamma, dbeta):
+            if t is not None:
+                t.zero_()
+        return dx
+    if x.is_cuda:
+        with nv.device_guard(x):
+            lib = nv.kernels()
+            ws = torch.empty(int(lib.dtf_groupnorm_workspace_floats(B, S, C, groups)), dtype=torch.float32, device=x.device)
+            rc = lib.dtf_groupnorm_bwd(nv.ptr(x), nv.ptr(dy), nv.ptr(dx), B, S, C, groups, _GROUPNORM_TYPES[x.dtype],
+                                       nv.ptr(gamma), nv.ptr(beta), int(act), nv.ptr(stats), nv.ptr(dgamma), nv.ptr(dbeta),
+                                       nv.ptr(ws), nv.stream_ptr())
+        nv.check(rc, "dtf_groupnorm_bwd")
+        return dx
+    xhat = _groupnorm_xhat(x, groups, stats)
+    u = xhat if gamma is None else xhat * gamma
+    u = u if beta is None else u + beta
+    if act == ACT_RELU:
+        slope = (u > 0).float()
+    elif act == ACT_SIGMOID:
+        slope = torch.sigmoid(u) * (1.0 - torch.sigmoid(u))
+    elif act == ACT_TANH:
+        slope = 1.0 - torch.tanh(u) ** 2
+    elif act == ACT_SILU:
+        slope = torch.sigmoid(u) * (1.0 + u * (1.0 - torch.sigmoid(u)))
+    else:
+        slope = torch.ones_like(u)
+    du = dy.float() * slope
+    lead = tuple(range(x.dim() - 1))
+    if dbeta is not None:
+        dbeta.copy_(du.sum(dim=lead, dtype=torch.float64))
+    if dgamma is not None:
+        dgamma.copy_((du * xhat).sum(dim=lead, dtype=torch.float64))
+    if dx is not None:
+        d = (du if gamma is None else du * gamma).view(B, S, groups, C // groups)
+        xg = xhat.view(B, S, groups, C // groups)
+        inv = stats[2].view(B, 1, groups, 1)
+        d = inv * (d - d.mean(dim=(1, 3), keepdim=True) - xg * (d * xg).mean(dim=(1, 3), keepdim=True))
+        dx.copy_(d.view(x.shape))
+    return dx
+
+
 def softmax(z, out=None):
     """Row softmax of logits [M, C]."""
     if out is None:
@@ -440,6 +570,121 @@ def softmax_xent(z, labels, grad_out=None, grad_scale=None, stats=None):
     return grad_out
 
 
+# --------------------------------------------------------------------------- softmax cross-entropy over a large vocabulary
+_XENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+#: what ``linear_xent_forward`` keeps for ``linear_xent_backward``; ``totals``: sum of the losses, counted rows, their mean
+LinearXentState = collections.namedtuple("LinearXentState", ["lse", "label_logit", "totals"])
+
+
+def _linear_xent_check(x, w, b, labels):
+    if x.dtype not in _XENT_TYPES or w.dtype != x.dtype or (b is not None and b.dtype != x.dtype):
+        raise ValueError("x, w and b must all be float32 or all bfloat16, got %s, %s, %s"
+                         % (x.dtype, w.dtype, None if b is None else b.dtype))
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[0] or x.shape[1] < 1 or w.shape[1] < 1:
+        raise ValueError("x [rows, features] and w [features, classes] do not fit: %s, %s" % (tuple(x.shape), tuple(w.shape)))
+    if b is not None and tuple(b.shape) != (w.shape[1],):
+        raise ValueError("b must have %d elements, got shape %s" % (w.shape[1], tuple(b.shape)))
+    if labels.dtype != torch.int64 or tuple(labels.shape) != (x.shape[0],):
+        raise ValueError("labels must be int64 of shape [%d], got %s %s" % (x.shape[0], labels.dtype, tuple(labels.shape)))
+    for t in (x, w, b, labels):
+        if t is not None and (t.device != x.device or not t.is_contiguous()):
+            raise ValueError("x, w, b and labels must be contiguous and on one device")
+
+
+def _linear_xent_logits(x, w, b, labels, ignore_index, bf16):
+    """Reference logits in float32; ignored rows count as zero rows of x."""
+    counted = labels != ignore_index
+    x32 = torch.where(counted.view(-1, 1), x.float(), torch.zeros((), dtype=torch.float32, device=x.device))
+    w32 = w.float()
+    if bf16:
+        x32, w32 = _bf16_round(x32), _bf16_round(w32)
+    z = x32 @ w32
+    return x32, w32, z if b is None else z + b.float(), counted
+
+
+def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False):
+    """Softmax cross-entropy of the logits ``x @ w + b`` (x [M, K], w [K, V], b [V] or None; all float32 or all bfloat16)
+    against int64 ``labels`` [M], for vocabularies whose [M, V] logits should not be in memory.
+
+    Rows with the label ``ignore_index`` count for nothing, whatever x holds there; any other label outside ``[0, V)`` makes
+    its row's loss NaN.  Classes may be masked by a ``b`` of -infinity.  ``bf16=True``: float32 operands are rounded to
+    bfloat16 for the products.  Returns ``(loss [M] float32, state)``; the state is what ``linear_xent_backward`` needs."""
+    _linear_xent_check(x, w, b, labels)
+    M, K, V = int(x.shape[0]), int(x.shape[1]), int(w.shape[1])
+    new = lambda n: torch.empty(n, dtype=torch.float32, device=x.device)
+    loss, state = new(M), LinearXentState(new(M), new(M), new(4))
+    if M == 0:
+        state.totals.zero_()
+        return loss, state
+    if x.is_cuda:
+        with nv.device_guard(x):
+            lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
+            ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(M, K, V, t, int(bf16))), dtype=torch.uint8,
+                             device=x.device)
+            rc = lib.dtf_linear_xent_fwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
+                                         int(ignore_index), nv.ptr(loss), nv.ptr(state.lse), nv.ptr(state.label_logit),
+                                         nv.ptr(state.totals), nv.ptr(ws), nv.stream_ptr())
+        nv.check(rc, "dtf_linear_xent_fwd")
+        return loss, state
+    _, _, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
+    state.lse.copy_(torch.logsumexp(z, dim=1))
+    valid = (labels >= 0) & (labels < V)
+    picked = z.gather(1, torch.where(valid, labels, torch.zeros_like(labels)).view(-1, 1)).view(-1)
+    state.label_logit.copy_(torch.where(valid, picked, torch.full_like(picked, float("nan"))))
+    loss.copy_(torch.where(counted, state.lse - state.label_logit, torch.zeros_like(loss)))
+    n = int(counted.sum())
+    state.totals.copy_(torch.tensor([float(loss.double().sum()), n, float(loss.double().sum()) / max(n, 1), 0.0]))
+    return loss, state
+
+
+def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index=-1, bf16=False, dx=None, dw=None, db=None):
+    """Gradient of ``linear_xent_forward`` into ``dx``, ``dw`` and ``db`` (like x, w and b; each may be None).
+
+    ``dloss`` float32: the gradient of every row's loss [M], or one value for all of them; ``mean=True`` divides it by the
+    number of counted rows (the gradient of their mean loss, ``state.totals[2]``)."""
+    _linear_xent_check(x, w, b, labels)
+    M, K, V = int(x.shape[0]), int(x.shape[1]), int(w.shape[1])
+    if dloss.dtype != torch.float32 or dloss.device != x.device or not dloss.is_contiguous() or dloss.numel() not in (1, M) \
+            or (dloss.numel() == 1) == (dloss.dim() == 1 and M != 1):
+        raise ValueError("dloss must be float32 [%d], or a single value of no dimension" % M)
+    for name, t, like in (("dx", dx, x), ("dw", dw, w), ("db", db, b)):
+        if t is not None and (like is None or t.dtype != like.dtype or t.shape != like.shape or t.device != x.device
+                              or not t.is_contiguous()):
+            raise ValueError("%s must be contiguous and like its operand" % name)
+    if M == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+        return
+    if x.is_cuda:
+        with nv.device_guard(x):
+            lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
+            ws = torch.empty(int(lib.dtf_linear_xent_bwd_workspace_bytes(M, K, V, t, int(bf16))), dtype=torch.uint8,
+                             device=x.device)
+            rc = lib.dtf_linear_xent_bwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
+                                         int(ignore_index), nv.ptr(state.lse), nv.ptr(state.label_logit), nv.ptr(state.totals),
+                                         int(bool(mean)), nv.ptr(dloss), int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw),
+                                         nv.ptr(db), nv.ptr(ws), nv.stream_ptr())
+        nv.check(rc, "dtf_linear_xent_bwd")
+        return
+    x32, w32, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
+    g = dloss.expand(M) / torch.clamp(state.totals[1], min=1.0) if mean else dloss.expand(M)
+    valid = (labels >= 0) & (labels < V)
+    g = torch.where(counted, torch.where(valid, g, torch.full_like(g, float("nan"))), torch.zeros_like(g))
+    dz = torch.exp(z - state.lse.view(-1, 1)) * g.view(-1, 1)
+    rows = torch.nonzero(valid).view(-1)
+    dz[rows, labels[rows]] = g[rows] * torch.expm1(state.label_logit[rows] - state.lse[rows])
+    dz = torch.where(counted.view(-1, 1), dz, torch.zeros_like(dz))
+    if db is not None:
+        db.copy_(dz.sum(dim=0))
+    if bf16:
+        dz = _bf16_round(dz)
+    if dx is not None:
+        dx.copy_(dz @ w32.t())
+    if dw is not None:
+        dw.copy_(x32.t() @ dz)
+
+
 def categorical_accuracy_sum(p, y, acc_sum):
     """acc_sum[0] += number of rows with argmax(p) == argmax(y) (Keras categorical_accuracy)."""
     M, N = p.shape
@@ -450,6 +695,83 @@ def categorical_accuracy_sum(p, y, acc_sum):
         return acc_sum
     acc_sum[0] += (p.argmax(dim=1) == y.argmax(dim=1)).to(torch.float32).sum()
     return acc_sum
+
+
+# --------------------------------------------------------------------------- global norm over a list of gradients
+_NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _norm_list(tensors):
+    """The list's tensors without its None entries, checked."""
+    live = [t for t in tensors if t is not None]
+    for t in live:
+        if t.dtype not in _NORM_TYPES or not t.is_contiguous() or t.device != live[0].device:
+            raise ValueError("the global norm takes contiguous float32, bfloat16 and float16 tensors on one device, got %s %s on %s"
+                             % (t.dtype, tuple(t.stride()), t.device))
+    return live
+
+
+def _norm_launch(live, dst, clip):
+    n = len(live)
+    with nv.device_guard(live[0]):
+        lib = nv.kernels()
+        partials = torch.empty(int(lib.dtf_global_norm_partials()), dtype=torch.float64, device=live[0].device)
+        norm = torch.empty((), dtype=torch.float32, device=live[0].device)
+        table = lambda kind, values: (kind * n)(*values)
+        rc = lib.dtf_global_norm(table(ctypes.c_longlong, [t.data_ptr() for t in live]),
+                                 None if dst is None else table(ctypes.c_longlong, [t.data_ptr() for t in dst]),
+                                 table(ctypes.c_longlong, [t.numel() for t in live]),
+                                 table(ctypes.c_byte, [_NORM_TYPES[t.dtype] for t in live]), n, float(clip), nv.ptr(partials),
+                                 nv.ptr(norm), nv.stream_ptr())
+    nv.check(rc, "dtf_global_norm")
+    return norm
+
+
+def global_norm(tensors):
+    """``tf.global_norm``: the square root of the sum of all squares over a list of tensors (float32, bfloat16, float16; None
+    entries count for nothing), as a float32 scalar tensor.  Summed in 64 bits and in a fixed order."""
+    live = _norm_list(tensors)
+    if not live:
+        return torch.zeros((), dtype=torch.float32)
+    if live[0].is_cuda:
+        return _norm_launch(live, None, math.inf)
+    return torch.stack([t.double().square().sum() for t in live]).sum().sqrt().float()
+
+
+def clip_by_global_norm(tensors, clip_norm, out=None):
+    """``tf.clip_by_global_norm``: ``([t * clip_norm / max(norm, clip_norm) for t in tensors], norm)`` with the global norm of
+    the unclipped list.  None entries stay None.  If the norm is not finite, every output is NaN.
+
+    ``out``: tensors to write into, like ``tensors`` (the list itself: in place, and nothing is written when nothing has to
+    be clipped); no two of them may share memory."""
+    clip_norm = float(clip_norm)
+    if not clip_norm > 0.0:
+        raise ValueError("clip_norm must be positive, got %r" % clip_norm)
+    tensors = list(tensors)
+    live = _norm_list(tensors)
+    if out is None:
+        out = [None if t is None else torch.empty_like(t) for t in tensors]
+    else:
+        out = list(out)
+        if len(out) != len(tensors) or any((o is None) != (t is None) for o, t in zip(out, tensors)):
+            raise ValueError("out must have a tensor for every tensor of the list")
+    dst = [o for o in out if o is not None]
+    for o, t in zip(dst, live):
+        if o.dtype != t.dtype or o.shape != t.shape or o.device != t.device or not o.is_contiguous():
+            raise ValueError("every tensor of out must be contiguous and like its tensor of the list")
+    spans = sorted((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size()) for o in dst if o.numel())
+    if any(a[1] > b[0] for a, b in zip(spans[:-1], spans[1:])):
+        raise ValueError("two tensors of out share memory")
+    if not live:
+        return out, torch.zeros((), dtype=torch.float32)
+    if live[0].is_cuda:
+        return out, _norm_launch(live, dst, clip_norm)
+    norm = torch.stack([t.double().square().sum() for t in live]).sum().sqrt()
+    v = float(norm)
+    f = math.nan if not math.isfinite(v) else 1.0 if v <= clip_norm else clip_norm / v
+    for o, t in zip(dst, live):
+        o.copy_((t.float() * f).to(t.dtype) if f != 1.0 else t)
+    return out, norm.float()
 
 
 # --------------------------------------------------------------------------- optimizers
