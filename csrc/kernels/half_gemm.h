@@ -1,0 +1,192 @@
+// Matrix products of 16-bit operands on the gfx950 matrix cores, as a main loop for kernels that bring their own epilogue:
+//
+//   acc[l, r] = sum_k L[l, k] R[r, k]          (fp32 accumulation)
+//
+// Each operand lies in memory either along k (rows l, k contiguous: "RC") or across it (rows k, l contiguous: "RS"), so no
+// operand is ever transposed in memory: RS tiles are read from LDS with the transposing 64-bit read.
+//
+// PL = 2 serves fp32 operands, kept as two fp16 limbs x = hi + lo (22 bits; what is lost is below fp32's own rounding of a
+// product): 32 values of a row are stored as 32 hi limbs, then 32 lo limbs, so that a tile of 2-limb values has the shape of
+// a tile of 16-bit values with half as many k.  Three limb products make one product: hi hi, hi lo, lo hi.
+//
+// A workgroup of WL x WR waves computes an LN x RN tile; a wave holds (LN / WL) x (RN / WR) of it in accumulators.  A stage is
+// 64 halves of the reduction an operand row: 128 bytes a row, loaded straight into LDS (16 bytes a lane); while one stage
+// is multiplied the next one arrives in the other buffer, one barrier a stage.
+//
+// LDS layouts.  RC: row of 128 bytes = 8 chunks of 16; chunk c of row i lies at c ^ (i & 7), so that the 32 rows that a
+// fragment read touches at one c spread over all banks.  RS: row k of LN * PL halves in granules of 32 bytes; granule q of
+// row k lies at q ^ 2 (k & 3): a transposing read takes 4 rows x 2 granules at once, which are then 8 distinct ones of 256 bytes.
+// The direct load writes LDS linearly, so the permutation is applied to the addresses it loads from.
+#pragma once
+#include "common.h"
+
+namespace hgemm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+template <typename H>
+struct Mma;
+template <>
+struct Mma<__bf16> {
+    static __device__ __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mma<_Float16> {
+    static __device__ __forceinline__ f32x16 run(s16x8 a, s16x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+typedef __attribute__((address_space(3))) char lds_char;
+
+// vectors at any element's address: global memory takes 16-byte accesses that are aligned to the element only
+typedef s16x8 s16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(unsigned, v);
+}
+
+// 32 accumulator columns of a row, times `g`, as bf16 at `out` (of this lane: 8 (lane >> 5) behind the row's first): a lane holds
+// 4 neighbours of every 8, its partner 32 lanes on the other 4; after the exchange each holds 8 of every 16 and writes 16 bytes.
+__device__ __forceinline__ void store_bf16_16(const f32x16& acc, float g, short* out, bool live) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        unsigned a0 = pack_bf16(acc[h * 8 + 0] * g, acc[h * 8 + 1] * g), a1 = pack_bf16(acc[h * 8 + 2] * g, acc[h * 8 + 3] * g);
+        unsigned b0 = pack_bf16(acc[h * 8 + 4] * g, acc[h * 8 + 5] * g), b1 = pack_bf16(acc[h * 8 + 6] * g, acc[h * 8 + 7] * g);
+        const auto p = __builtin_amdgcn_permlane32_swap(a0, b0, false, false), q = __builtin_amdgcn_permlane32_swap(a1, b1, false, false);
+        typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4 v = {p[0], q[0], p[1], q[1]};
+        if (live) *reinterpret_cast<s16x8_any*>(out + h * 16) = __builtin_bit_cast(s16x8, v);
+    }
+}
+
+// One operand's tile in memory: `base` is its first element, `left` the bytes from there to the end of the operand (what lies
+// behind reads as zero), `ld` the bytes of a row.
+struct Tile {
+    const char* base;
+    long long left, ld;
+};
+
+template <typename H, int PL, int LN, int RN, int WL, int WR, bool L_RS, bool R_RS>
+struct Gemm {
+    static constexpr int THREADS = 64 * WL * WR, WAVES = WL * WR;
+    static constexpr int CB = 64 / PL;                       // values of the reduction a stage
+    static constexpr int TL = LN / WL / 32, TR = RN / WR / 32;
+    static constexpr int L_BYTES = LN * 128, R_BYTES = RN * 128, STAGE = L_BYTES + R_BYTES;
+    static constexpr int LDS_BYTES = 2 * STAGE;
+    static constexpr int KS = CB / 16;                       // MFMA steps a stage and limb product
+    static_assert(LN % (32 * WL) == 0 && RN % (32 * WR) == 0 && (LN / 8) % WAVES == 0 && (RN / 8) % WAVES == 0, "tile");
+    static_assert((!L_RS || LN == 256) && (!R_RS || RN == 256), "the RS layout's banks are worked out for rows of 256 values");
+
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const char* base, long long left) {
+        const long long n = left < 0 ? 0 : left > 0xffffffffll ? 0xffffffffll : left;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)(unsigned)n, 0x00020000);
+    }
+
+    // LDS <- stage `blk` of one operand
+    template <int N, bool RS>
+    static __device__ __forceinline__ void load(const Tile& t, int blk, lds_char* dst) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        constexpr int LOADS = N / 8 / WAVES;                 // 1 KB each
+        if (!RS) {
+            const __amdgpu_buffer_rsrc_t rs = resource(t.base + (long long)blk * 128, t.left - (long long)blk * 128);
+            const unsigned ld = (unsigned)t.ld;
+            unsigned off = (unsigned)(wave * LOADS * 8 + (lane >> 3)) * ld + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
+                                                         (int)off, 0, 0, 0);
+                off += 8 * ld;
+            }
+        } else {
+            constexpr int SLOTS = N * PL / 8;                // 16-byte chunks a row: 32 or 64
+            constexpr int ROWS = 64 / SLOTS;                 // rows a load: 2 or 1
+            const long long skip = (long long)blk * CB * t.ld;
+            const __amdgpu_buffer_rsrc_t rs = resource(t.base + skip, t.left - skip);
+            const unsigned ld = (unsigned)t.ld;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int row = (wave * LOADS + i) * ROWS + lane / SLOTS;
+                const int chunk = (lane % SLOTS) ^ (4 * (row & 3));
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
+                                                         (int)((unsigned)row * ld + (unsigned)chunk * 16), 0, 0, 0);
+            }
+        }
+    }
+
+    // Fragment of 32 values x 16 steps of k: lane holds value lane & 31, steps 8 (lane >> 5) ... + 7.
+    template <bool RS, int N>
+    static __device__ __forceinline__ s16x8 frag(const lds_char* src, int tile32, int plane, int kk) {
+        const int lane = threadIdx.x & 63;
+        if (!RS) {
+            const int chunk = plane * 4 + kk * 2 + (lane >> 5);
+            return *(const __attribute__((address_space(3))) s16x8*)(src + (tile32 * 32 + (lane & 31)) * 128 + ((chunk ^ (lane & 7)) * 16));
+        }
+        constexpr int ROW = N * PL * 2;
+        const int granule = tile32 * 2 * PL + plane * 2 + ((lane >> 4) & 1);
+        const int row = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
+        const lds_char* p = src + row * ROW + ((granule ^ (2 * ((lane >> 2) & 3))) * 32) + (lane & 3) * 8;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * ROW));
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+
+    // One stage multiplied from `now` while stage `blk` (if `more`) is loaded into `next`.  The two buffers are told apart by
+    // __restrict__: without it the compiler waits for the loads into `next` before the first read of `now`.
+    static __device__ __forceinline__ void step(const Tile& tl, const Tile& tr, int blk, bool more, const lds_char* __restrict__ now,
+                                                lds_char* __restrict__ next, int wl, int wr, f32x16 (&acc)[TL][TR]) {
+        if (more) {
+            load<LN, L_RS>(tl, blk, next);
+            load<RN, R_RS>(tr, blk, next + L_BYTES);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            s16x8 fl[PL][TL], fr[PL][TR];
+#pragma unroll
+            for (int p = 0; p < PL; ++p) {
+#pragma unroll
+                for (int a = 0; a < TL; ++a) fl[p][a] = frag<L_RS, LN>(now, wl * TL + a, p, kk);
+#pragma unroll
+                for (int b = 0; b < TR; ++b) fr[p][b] = frag<R_RS, RN>(now + L_BYTES, wr * TR + b, p, kk);
+            }
+#pragma unroll
+            for (int a = 0; a < TL; ++a)
+#pragma unroll
+                for (int b = 0; b < TR; ++b) {
+                    if (PL == 2) {
+                        acc[a][b] = Mma<H>::run(fr[PL - 1][b], fl[0][a], acc[a][b]);
+                        acc[a][b] = Mma<H>::run(fr[0][b], fl[PL - 1][a], acc[a][b]);
+                    }
+                    acc[a][b] = Mma<H>::run(fr[0][b], fl[0][a], acc[a][b]);
+                }
+        }
+    }
+
+    static __device__ __forceinline__ void run(const Tile& tl, const Tile& tr, int blocks, lds_char* smem, f32x16 (&acc)[TL][TR]) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wl = wave / WR, wr = wave % WR;
+#pragma unroll
+        for (int a = 0; a < TL; ++a)
+#pragma unroll
+            for (int b = 0; b < TR; ++b) acc[a][b] = f32x16{};
+        if (blocks <= 0) return;
+        load<LN, L_RS>(tl, 0, smem);
+        load<RN, R_RS>(tr, 0, smem + L_BYTES);
+        for (int blk = 0; blk < blocks; ++blk) {
+            // this wave's loads of the stage are in LDS; then everybody's are, and everybody is done with the other buffer
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            step(tl, tr, blk + 1, blk + 1 < blocks, smem + (blk & 1) * STAGE, smem + ((blk + 1) & 1) * STAGE, wl, wr, acc);
+        }
+    }
+};
+
+}  // namespace hgemm

@@ -3,314 +3,923 @@
 //   lse_m = log sum_v exp z_mv;   loss_m = lse_m - z_m,label;   rows whose label is `ignore` count for nothing
 //   dz = g_m (exp(z - lse) - onehot);   dx = dz w^T;   dw = x^T dz;   db = sum_m dz
 //
-// The vocabulary is taken in pieces: the forward pass keeps a running maximum and sum of every row, the backward pass computes
-// a piece's logits again and turns them into the piece's dz at once.
+// Forward: one matrix product whose tiles (256 classes wide) never leave registers as logits: a tile leaves every row's maximum,
+// its sum of exponentials and, where the label falls into it, the label's logit.  A second kernel joins the tiles' pairs.
+//
+// Backward, a piece of the vocabulary at a time: e = exp(z - tile maximum) of the piece -> dz of the piece -> its part of dx
+// (added up in fp32 over pieces and splits) and its columns of dw, whole.  Where the forward pass was told to, it has kept e
+// for the first `kept` classes (as many as fit the caller's memory budget); the logits of the others are computed again.
+// With everything kept a training step is the three products that it cannot do without.
+//
+// Numbers.  bf16 operands multiply as they are.  fp32 operands are scaled by a power of two for each tensor (largest value
+// in [2^14, 2^15)) and split into two fp16 limbs of 22 bits together, multiplied as three limb products (half_gemm.h): as exact
+// as fp32 products, at a third of the fp16 rate instead of the sixteenth that fp32 matrix instructions have.  All sums and
+// softmax statistics are fp32 or wider.  e is kept in bf16 for bf16 operands: one rounding of a factor of dz, which is rounded
+// to bf16 for its products anyway; fp32 for fp32.  dz is held in units of a power of two, and without the loss's gradient where
+// that is one number for all rows: (p - 1) at a label is then near -1, which bf16 holds well, instead of the same rounding error in every row; and at the
+// label it comes from expm1(z_label - lse), not from a rounded p.
 //
 // Masked classes (b = -infinity or the type's lowest value) get probability zero.  A label outside [0, V) that is not `ignore`
-// makes the row's loss and gradients NaN.  x may hold anything in ignored rows.
+// makes the row's loss and gradients NaN.  x may hold anything in ignored rows: it is packed as zeros there.
 #include "common.h"
+#include "half_gemm.h"
 
 #include <hip/hip_bf16.h>
 
 namespace {
 
-constexpr int XT = 64, XK = 16;          // output tile 64 x 64, 16 steps of the reduction in LDS
+using hgemm::Gemm;
+using hgemm::lds_char;
+using hgemm::s16x8;
+using hgemm::Tile;
+
+constexpr int XT = 256;                          // classes a tile
+constexpr long long XE_PIECE_BYTES = 128ll << 20; // dz of a piece: stays in the 256 MB cache between its kernels
+constexpr long long XE_PACK_BYTES = 256ll << 20;  // w of a piece where it has to be packed
+constexpr float XE_DZ_SCALE = 16384.f;           // what dz, below 2 in its units, is multiplied by before it is split
+
+template <int PL>
+struct HalfOf {
+    typedef __bf16 type;
+};
+template <>
+struct HalfOf<2> {
+    typedef _Float16 type;
+};
 
 __device__ __forceinline__ float xe_load(const float* p) { return *p; }
 __device__ __forceinline__ float xe_load(const __hip_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void xe_store(float* p, float v) { *p = v; }
-__device__ __forceinline__ void xe_store(__hip_bfloat16* p, float v) { *p = __float2bfloat16(v); }
-__device__ __forceinline__ float xe_round(float v, int bf16) { return bf16 ? __bfloat162float(__float2bfloat16(v)) : v; }
+__device__ __forceinline__ short xe_bf16(float v) {
+    const __hip_bfloat16 h = __float2bfloat16(v);
+    return __builtin_bit_cast(short, h);
+}
 
-// C tile (64 x 64) of A B with A(i, r) and B(r, j) given as functions; thread (ty, tx) holds rows ty + 16 a, columns tx + 16 c
-template <typename FA, typename FB>
-__device__ __forceinline__ void xe_tile(FA a_at, FB b_at, long long R, float (&acc)[4][4]) {
-    __shared__ float as[XK][XT + 1], bs[XK][XT + 1];
-    const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+// power of two that brings a largest magnitude (its bits) into [2^14, 2^15), and its inverse
+__device__ __forceinline__ float xe_scale(unsigned amax_bits) {
+    const int e = (int)(amax_bits >> 23);                       // biased exponent; subnormal maxima count as the smallest normal
+    const int s = 127 + 14 - ((e < 1 ? 1 : e) - 127);
+    return amax_bits == 0 ? 1.f : __uint_as_float((unsigned)(s > 253 ? 253 : s) << 23);
+}
+
+// ---- scales: the largest finite magnitudes of x (counted rows) and w, as bits
+__global__ void xe_zero_kernel(unsigned* __restrict__ amax) { amax[threadIdx.x] = 0u; }
+
+__global__ __launch_bounds__(256) void xe_amax_kernel(const float* __restrict__ X, long long M, long long K,
+                                                      const long long* __restrict__ labels, long long ignore,
+                                                      const float* __restrict__ W, long long KV, unsigned* __restrict__ amax) {
+    const bool is_x = blockIdx.y == 0;
+    const float* p = is_x ? X : W;
+    const long long n = is_x ? M * K : KV;
+    float m = 0.f;
+    const long long stride = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const float v = fabsf(p[i]);
+        if (v < __builtin_inff() && (!is_x || labels[i / K] != ignore)) m = fmaxf(m, v);
+    }
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(amax + (is_x ? 0 : 1), __float_as_uint(m));   // order does not matter
+}
+
+// ---- packing: [rows, cols] of any alignment -> rows of ld halves, zero behind cols; rows labelled `ignore` as zeros
+template <typename T, int PL>
+__global__ __launch_bounds__(256) void xe_pack_kernel(const T* __restrict__ src, long long ld_src, long long rows, long long cols,
+                                                      short* __restrict__ dst, long long ld, const long long* __restrict__ labels,
+                                                      long long ignore, const unsigned* __restrict__ amax, int vec) {
+    const long long per_row = ld / PL / 8;                      // groups of 8 values
+    const long long total = rows * per_row;
+    const float scale = PL == 2 ? xe_scale(*amax) : 1.f;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / per_row, c = (i - r * per_row) * 8;
+        float v[8];
+        const bool skip = labels && labels[r] == ignore;
+        const T* p = src + r * ld_src + c;
+        if (vec && c + 8 <= cols && !skip) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) acc[a][c] = 0.f;
-    for (long long r0 = 0; r0 < R; r0 += XK) {
-        __syncthreads();
-        for (int e = tid; e < XK * XT; e += 256) {
-            const int r = e / XT, i = e % XT;
-            as[r][i] = r0 + r < R ? a_at(i, r0 + r) : 0.f;
-            bs[r][i] = r0 + r < R ? b_at(r0 + r, i) : 0.f;
+            for (int e = 0; e < 8; e += 16 / (int)sizeof(T)) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(p + e);
+                const T* t = reinterpret_cast<const T*>(&q);
+#pragma unroll
+                for (int j = 0; j < 16 / (int)sizeof(T); ++j) v[e + j] = xe_load(t + j);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = !skip && c + e < cols ? xe_load(p + e) : 0.f;
         }
-        __syncthreads();
+        s16x8 hi, lo;
 #pragma unroll
-        for (int r = 0; r < XK; ++r)
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) acc[a][c] = fmaf(as[r][ty + 16 * a], bs[r][tx + 16 * c], acc[a][c]);
+        for (int e = 0; e < 8; ++e) {
+            if (PL == 1) {
+                hi[e] = xe_bf16(v[e]);
+            } else {
+                const float s = v[e] * scale;
+                const _Float16 h = (_Float16)s;
+                const _Float16 l = fabsf((float)h) < __builtin_inff() ? (_Float16)(s - (float)h) : (_Float16)0.f;
+                hi[e] = __builtin_bit_cast(short, h);
+                lo[e] = __builtin_bit_cast(short, l);
+            }
+        }
+        short* q = dst + r * ld + (PL == 1 ? c : c / 32 * 64 + c % 32);
+        *reinterpret_cast<s16x8*>(q) = hi;
+        if (PL == 2) *reinterpret_cast<s16x8*>(q + 32) = lo;
     }
 }
 
-// Logits of a 64 x 64 tile.  DZ false: the tile's maximum and sum of exponentials of every row, the label's logit.
-// DZ true: dz into the piece's buffer [M, ld] (columns from v0).
-template <typename T, bool DZ>
-__global__ __launch_bounds__(256) void xe_logits_kernel(const T* __restrict__ X, const T* __restrict__ W, const T* __restrict__ Bv,
-                                                        const long long* __restrict__ labels, long long M, long long K, long long V,
-                                                        long long v0, long long vend, int bf16, long long ignore,
-                                                        float* __restrict__ tmax, float* __restrict__ tsum, long long ntiles,
-                                                        float* __restrict__ zlab, const float* __restrict__ lse,
-                                                        const float* __restrict__ dloss, int dloss_stride,
-                                                        const float* __restrict__ totals, int mean, float* __restrict__ dz,
-                                                        long long ld) {
-    __shared__ float zt[XT][XT + 1];
-    const long long m0 = (long long)blockIdx.y * XT, n0 = v0 + (long long)blockIdx.x * XT;
-    float acc[4][4];
-    auto a_at = [&](int i, long long r) -> float {
+// Workgroup -> tile.  Workgroups go round the 8 XCDs one after another: each XCD gets a contiguous run of tiles, and within it
+// tiles run down 8 rows of tiles before they move to the next column, so that the operands of neighbours meet in its L2.
+__device__ __forceinline__ void xe_tile_of(long long bid, long long count, long long nrow, long long ncol, long long& row, long long& col) {
+    const long long x = bid & 7, base = count >> 3, extra = count & 7;
+    const long long t = x * base + (x < extra ? x : extra) + (bid >> 3);
+    const long long group = t / (8 * ncol), first = group * 8;
+    const long long rows = nrow - first < 8 ? nrow - first : 8;
+    const long long in = t - group * 8 * ncol;
+    row = first + in % rows;
+    col = in / rows;
+}
+
+// ---- logits of an LN x 256 tile and what the softmax needs of them
+template <int PL, int LN, int WL, int WR>
+__global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
+    const short* __restrict__ X, long long ldx, const short* __restrict__ W, long long ldw, long long w_left,
+    const void* __restrict__ bias, int bias_bf16, const long long* __restrict__ labels, long long M, long long K, long long v0,
+    long long vend, const unsigned* __restrict__ amax, float* __restrict__ tmax, float* __restrict__ tsum,
+    float* __restrict__ zlab, float* __restrict__ beaten, void* __restrict__ E, long long lde, long long e0, long long e_tiles) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const long long nrow = (M + LN - 1) / LN, ncol = (vend - v0 + XT - 1) / XT;
+    long long rt, ct;
+    xe_tile_of(blockIdx.x, nrow * ncol, nrow, ncol, rt, ct);
+    const long long m0 = rt * LN, n0 = ct * XT;                 // n0 within the piece
+    const Tile tl = {reinterpret_cast<const char*>(X + m0 * ldx), (M - m0) * ldx * 2, ldx * 2};
+    const Tile tr = {reinterpret_cast<const char*>(W + n0 * PL), w_left - n0 * PL * 2, ldw * 2};
+    f32x16 acc[G::TL][G::TR];
+    G::run(tl, tr, (int)(ldx / 64), (lds_char*)smem, acc);
+    __syncthreads();
+
+    float* sbias = reinterpret_cast<float*>(smem);              // [256]
+    float* smax = sbias + XT;                                   // [WR][LN]
+    float* ssum = smax + WR * LN;                               // [WR][LN]
+    float* slab = ssum + WR * LN;                               // [LN]: the labels' logits
+    unsigned* sbeat = reinterpret_cast<unsigned*>(slab + LN);   // [LN]
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wl = wave / WR, wr = wave % WR;
+    for (int i = tid; i < XT; i += G::THREADS) {
+        const long long n = v0 + n0 + i;
+        sbias[i] = n >= vend ? -__builtin_inff() : !bias ? 0.f : bias_bf16 ? xe_load(static_cast<const __hip_bfloat16*>(bias) + n)
+                                                                            : static_cast<const float*>(bias)[n];
+    }
+    for (int i = tid; i < LN; i += G::THREADS) sbeat[i] = 0u;
+    __syncthreads();
+    const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) : 1.f, iw = PL == 2 ? 1.f / xe_scale(amax[1]) : 1.f;
+    const bool full = v0 + n0 + XT <= vend;
+    const int nw = wr * (XT / WR) + 4 * (lane >> 5);            // first class of this lane's, within the tile
+    int own[G::TL];                                             // the row's label within the tile, or out of it
+    bool any_own = false;
+#pragma unroll
+    for (int a = 0; a < G::TL; ++a) {
+        const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
+        const long long l = m0 + ml < M ? labels[m0 + ml] - v0 - n0 : -1;
+        own[a] = l >= 0 && l < XT && v0 + n0 + l < vend ? (int)l : -1;
+        any_own |= own[a] >= 0;
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 bz = *reinterpret_cast<const f32x4*>(sbias + nw + b * 32 + q * 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float z = acc[a][b][q * 4 + i];
+                    if (PL == 2) z = z * ix * iw;
+                    z = full || v0 + n0 + nw + b * 32 + q * 8 + i < vend ? z + bz[i] : -__builtin_inff();
+                    acc[a][b][q * 4 + i] = z;
+                    mx = fmaxf(mx, z);
+                }
+            }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        if (lane < 32) smax[wr * LN + ml] = mx;
+    }
+    any_own = __any(any_own);
+    if (any_own) {                                              // few tiles hold any label of their rows
+#pragma unroll
+        for (int a = 0; a < G::TL; ++a)
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (nw + b * 32 + (r >> 2) * 8 + (r & 3) == own[a]) slab[wl * (LN / WL) + a * 32 + (lane & 31)] = acc[a][b][r];
+    }
+    __syncthreads();
+    const bool keep = E && ct < e_tiles;
+#pragma unroll
+    for (int a = 0; a < G::TL; ++a) {
+        const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
+        float mx = smax[ml];
+#pragma unroll
+        for (int w = 1; w < WR; ++w) mx = fmaxf(mx, smax[w * LN + ml]);
+        const float shift = mx == -__builtin_inff() ? 0.f : mx;
+        float s = 0.f;
+        if (any_own && own[a] >= 0) {                           // does another class of the tile beat the label's?
+            const float zl = slab[ml];
+            bool beat = false;
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float z = acc[a][b][r];
+                    beat |= z > zl || (z == zl && nw + b * 32 + (r >> 2) * 8 + (r & 3) < own[a]);
+                }
+            if (beat) sbeat[ml] = 1u;                           // all write the same
+        }
+#pragma unroll
+        for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __expf(acc[a][b][r] - shift);
+                acc[a][b][r] = e;
+                s += e;
+            }
+        s += __shfl_xor(s, 32, 64);
+        if (lane < 32) ssum[wr * LN + ml] = s;
+        if (keep && m0 + ml < M) {
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b) {
+                if (PL == 2) {
+                    float* out = static_cast<float*>(E) + (m0 + ml) * lde + e0 + n0 + nw + b * 32;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<f32x4*>(out + q * 8) =
+                            f32x4{acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
+                }
+            }
+        }
+        if (PL == 1 && keep) {
+            short* out = static_cast<short*>(E) + (m0 + ml) * lde + e0 + n0 + wr * (XT / WR) + 8 * (lane >> 5);
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b) hgemm::store_bf16_16(acc[a][b], 1.f, out + b * 32, m0 + ml < M);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < LN; i += G::THREADS) {
         const long long m = m0 + i;
-        return m < M && labels[m] != ignore ? xe_round(xe_load(X + m * K + r), bf16) : 0.f;
-    };
-    auto b_at = [&](long long r, int j) -> float { return n0 + j < vend ? xe_round(xe_load(W + r * V + n0 + j), bf16) : 0.f; };
-    xe_tile(a_at, b_at, K, acc);
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+        if (m >= M) continue;
+        float mx = smax[i], s = ssum[i];
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const long long n = n0 + tx + 16 * c;
-            zt[ty + 16 * a][tx + 16 * c] = n < vend ? acc[a][c] + (Bv ? xe_load(Bv + n) : 0.f) : -__builtin_inff();
+        for (int w = 1; w < WR; ++w) {
+            mx = fmaxf(mx, smax[w * LN + i]);
+            s += ssum[w * LN + i];
+        }
+        const long long tile = v0 / XT + ct;
+        if (tsum) {
+            tmax[tile * M + m] = mx;
+            tsum[tile * M + m] = s;
+            const long long l = labels[m] - v0 - n0;
+            if (l >= 0 && l < XT && v0 + n0 + l < vend) {
+                zlab[m] = slab[i];
+                beaten[m] = sbeat[i] ? 1.f : 0.f;
+            }
+        }
+    }
+}
+
+// ---- the tiles' maxima and sums joined: lse, loss, whether the label has the largest logit (ties to the lowest class).
+// A workgroup takes `rows` rows (a power of two up to 64), 256 / rows threads a row.
+__global__ __launch_bounds__(256) void xe_merge_kernel(const float* __restrict__ tmax, const float* __restrict__ tsum, long long ntiles,
+                                                       const long long* __restrict__ labels, long long M, long long V, long long ignore,
+                                                       int rows, const float* __restrict__ zlab, const float* __restrict__ beaten,
+                                                       float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ hit) {
+    __shared__ float red[256];
+    const int lanes = 256 / rows, rl = threadIdx.x % rows, tl = threadIdx.x / rows;
+    const long long m = (long long)blockIdx.x * rows + rl;
+    const bool live = m < M;
+    float mx = -__builtin_inff();
+    if (live)
+        for (long long t = tl; t < ntiles; t += lanes) mx = fmaxf(mx, tmax[t * M + m]);
+    red[threadIdx.x] = mx;
+    __syncthreads();
+    for (int k = 0; k < lanes; ++k) mx = fmaxf(mx, red[k * rows + rl]);
+    float s = 0.f;
+    const long long label = live ? labels[m] : ignore;
+    const bool valid = live && label >= 0 && label < V;
+    const float zl = valid ? zlab[m] : 0.f;
+    float lost = 0.f;
+    if (live)
+        for (long long t = tl; t < ntiles; t += lanes) {
+            const float v = tmax[t * M + m];
+            s += tsum[t * M + m] * __expf(v - mx);
+            if (t != label / XT && (v > zl || (v == zl && t < label / XT))) lost = 1.f;
         }
     __syncthreads();
-    if (!DZ) {
-        const long long m = m0 + threadIdx.x;
-        if (threadIdx.x < XT && m < M) {
-            float mx = -__builtin_inff(), s = 0.f;
-            for (int j = 0; j < XT; ++j) {
-                const float z = zt[threadIdx.x][j];
-                mx = z > mx || z != z ? z : mx;
-            }
-            const float shift = mx == -__builtin_inff() ? 0.f : mx;
-            for (int j = 0; j < XT; ++j) s += __expf(zt[threadIdx.x][j] - shift);
-            const long long tile = (v0 / XT) + blockIdx.x;
-            tmax[m * ntiles + tile] = mx;
-            tsum[m * ntiles + tile] = s;
-            const long long l = labels[m];
-            if (l >= n0 && l < n0 + XT && l < vend) zlab[m] = zt[threadIdx.x][l - n0];
-        }
-    } else {
-        for (int e = threadIdx.x; e < XT * XT; e += 256) {
-            const int i = e / XT, j = e % XT;
-            const long long m = m0 + i, n = n0 + j;
-            if (m >= M || n >= vend) continue;
-            const long long l = labels[m];
-            float g = dloss[m * dloss_stride] * (mean ? 1.f / fmaxf(totals[1], 1.f) : 1.f);
-            float d = 0.f;
-            if (l != ignore) {
-                if (l < 0 || l >= V) g = __builtin_nanf("");
-                d = g * (n == l ? expm1f(zt[i][j] - lse[m]) : __expf(zt[i][j] - lse[m]));
-            }
-            dz[m * ld + (n - v0)] = xe_round(d, bf16);
-        }
-    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    s = 0.f;
+    for (int k = 0; k < lanes; ++k) s += red[k * rows + rl];
+    __syncthreads();
+    red[threadIdx.x] = lost;
+    __syncthreads();
+    if (tl != 0 || !live) return;
+    for (int k = 1; k < lanes; ++k) lost += red[k * rows + rl];
+    const float l = mx + logf(s);
+    lse[m] = l;
+    loss[m] = label == ignore ? 0.f : valid ? l - zl : __builtin_nanf("");
+    hit[m] = label != ignore && valid && lost == 0.f && beaten[m] == 0.f ? 1.f : 0.f;
 }
 
-// One wave per row: the tiles' maxima and sums joined; lse and loss.
-__global__ __launch_bounds__(64) void xe_merge_kernel(const float* __restrict__ tmax, const float* __restrict__ tsum,
-                                                      long long ntiles, const long long* __restrict__ labels, long long V,
-                                                      long long ignore, const float* __restrict__ zlab, float* __restrict__ lse,
-                                                      float* __restrict__ loss) {
-    const long long m = blockIdx.x;
-    float mx = -__builtin_inff();
-    bool bad = false;
-    for (long long t = threadIdx.x; t < ntiles; t += 64) {
-        const float v = tmax[m * ntiles + t];
-        bad |= v != v;
-        mx = fmaxf(mx, v);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-    float s = 0.f;
-    for (long long t = threadIdx.x; t < ntiles; t += 64) {
-        const float v = tmax[m * ntiles + t];
-        if (v != -__builtin_inff()) s += tsum[m * ntiles + t] * __expf(v - mx);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (__any(bad)) s = __builtin_nanf("");
-    if (threadIdx.x == 0) {
-        const float l = mx + __logf(s);
-        lse[m] = l;
-        const long long at = labels[m];
-        loss[m] = at == ignore ? 0.f : at < 0 || at >= V ? __builtin_nanf("") : l - zlab[m];
-    }
-}
-
-// totals: sum of the losses, counted rows, mean over the counted rows (0 where there are none).  One workgroup, fixed order.
-__global__ __launch_bounds__(256) void xe_total_kernel(const float* __restrict__ loss, const long long* __restrict__ labels,
-                                                       long long M, long long ignore, float* __restrict__ totals) {
-    __shared__ double part[2][256];
-    double s = 0.0, n = 0.0;
-    for (long long m = threadIdx.x; m < M; m += 256) {
+// totals: sum of the losses, counted rows, mean over the counted rows (0 where there are none), hits.  One workgroup, fixed order.
+__global__ __launch_bounds__(1024) void xe_total_kernel(const float* __restrict__ loss, const float* __restrict__ hit,
+                                                        const long long* __restrict__ labels, long long M, long long ignore,
+                                                        float* __restrict__ totals) {
+    __shared__ double part[3][16];
+    double s = 0.0, n = 0.0, h = 0.0;
+    for (long long m = threadIdx.x; m < M; m += 1024) {
         s += (double)loss[m];
+        h += (double)hit[m];
         n += labels[m] != ignore ? 1.0 : 0.0;
     }
-    part[0][threadIdx.x] = s;
-    part[1][threadIdx.x] = n;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o, 64);
+        n += __shfl_xor(n, o, 64);
+        h += __shfl_xor(h, o, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        part[0][threadIdx.x >> 6] = s;
+        part[1][threadIdx.x >> 6] = n;
+        part[2][threadIdx.x >> 6] = h;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int k = 1; k < 256; ++k) {
+        s = n = h = 0.0;
+        for (int k = 0; k < 16; ++k) {
             s += part[0][k];
             n += part[1][k];
+            h += part[2][k];
         }
         totals[0] = (float)s;
         totals[1] = (float)n;
         totals[2] = (float)(s / fmax(n, 1.0));
+        totals[3] = (float)h;
     }
 }
 
-// dx32 [M, K] (+)= dz [M, cols] w[:, v0 ...]^T
-template <typename T>
-__global__ __launch_bounds__(256) void xe_dx_kernel(const float* __restrict__ dz, long long ld, const T* __restrict__ W, long long M,
-                                                    long long K, long long V, long long v0, long long cols, int bf16, int first,
-                                                    int last, float* __restrict__ dx32, T* __restrict__ DX) {
-    const long long m0 = (long long)blockIdx.y * XT, k0 = (long long)blockIdx.x * XT;
-    float acc[4][4];
-    auto a_at = [&](int i, long long r) -> float { return m0 + i < M ? dz[(m0 + i) * ld + r] : 0.f; };
-    auto b_at = [&](long long r, int j) -> float { return k0 + j < K ? xe_round(xe_load(W + (k0 + j) * V + v0 + r), bf16) : 0.f; };
-    xe_tile(a_at, b_at, cols, acc);
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+// ---- weights of the rows, one workgroup: rowg[m] *scale = the gradient of row m's loss.
+// The largest |dz| of a row is 1 - p_label (the other probabilities add up to it).  *scale holds the power of two of the largest
+// one over all rows, so that dz / *scale is below 2 and near 1 somewhere, also where every row is confident: fp16 limbs resolve
+// 2^-39 of that.
+__global__ __launch_bounds__(1024) void xe_weights_kernel(const float* __restrict__ dloss, int stride, const float* __restrict__ totals,
+                                                          int mean, const long long* __restrict__ labels, long long M, long long V,
+                                                          long long ignore, const float* __restrict__ lse, const float* __restrict__ zlab,
+                                                          float* __restrict__ rowg, float* __restrict__ scale) {
+    __shared__ float part[16];
+    float m = 0.f;
+    for (long long i = threadIdx.x; i < M; i += 1024) {
+        const long long l = labels[i];
+        const bool valid = l != ignore && l >= 0 && l < V;
+        const float w = stride ? dloss[i] : 1.f;
+        rowg[i] = l == ignore ? 0.f : valid ? w : __builtin_nanf("");
+        const float d = valid ? fabsf(w * expm1f(zlab[i] - lse[i])) : 0.f;
+        if (d < __builtin_inff()) m = fmaxf(m, d);
+    }
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const long long m = m0 + ty + 16 * a, k = k0 + tx + 16 * c;
-            if (m >= M || k >= K) continue;
-            const float v = acc[a][c] + (first ? 0.f : dx32[m * K + k]);
-            if (last) xe_store(DX + m * K + k, v);
-            else dx32[m * K + k] = v;
-        }
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = part[0];
+    for (int k = 1; k < 16; ++k) m = fmaxf(m, part[k]);
+    const int e = (int)(__float_as_uint(m) >> 23) - 127;
+    const int unit = m == 0.f ? 0 : e < -100 ? -100 : e > 100 ? 100 : e;
+    const float down = __uint_as_float((unsigned)(127 - unit) << 23);
+    for (long long i = threadIdx.x; i < M; i += 1024) rowg[i] *= down;
+    if (threadIdx.x == 0)
+        *scale = (stride ? 1.f : *dloss) * (mean ? 1.f / fmaxf(totals[1], 1.f) : 1.f) * __uint_as_float((unsigned)(127 + unit) << 23);
 }
 
-// dw[:, v0 ...] = x^T dz; x counts as zero in ignored rows
-template <typename T>
-__global__ __launch_bounds__(256) void xe_dw_kernel(const T* __restrict__ X, const float* __restrict__ dz, long long ld,
-                                                    const long long* __restrict__ labels, long long M, long long K, long long V,
-                                                    long long v0, long long cols, int bf16, long long ignore, T* __restrict__ DW) {
-    const long long k0 = (long long)blockIdx.y * XT, n0 = (long long)blockIdx.x * XT;
-    float acc[4][4];
-    auto a_at = [&](int i, long long r) -> float {
-        return k0 + i < K && labels[r] != ignore ? xe_round(xe_load(X + r * K + k0 + i), bf16) : 0.f;
-    };
-    auto b_at = [&](long long r, int j) -> float { return n0 + j < cols ? dz[r * ld + n0 + j] : 0.f; };
-    xe_tile(a_at, b_at, M, acc);
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+// ---- e of a piece -> its dz, 64 rows x 256 classes a workgroup; dbp [row blocks][ld]: the columns' sums over the 64 rows
+template <int PL>
+__global__ __launch_bounds__(256) void xe_dz_kernel(const void* __restrict__ E, long long lde, long long e0,
+                                                    const float* __restrict__ tmax, const float* __restrict__ lse,
+                                                    const float* __restrict__ zlab, const float* __restrict__ rowg,
+                                                    const long long* __restrict__ labels, long long M, long long v0,
+                                                    short* __restrict__ dz, long long ld, float* __restrict__ dbp) {
+    __shared__ float f[64], at_label[64];
+    __shared__ int own[64];
+    __shared__ float sums[8][XT];
+    const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * XT;
+    if (threadIdx.x < 64) {
+        const long long m = m0 + threadIdx.x;
+        const float g = m < M ? rowg[m] : 0.f;
+        const float mx = m < M ? tmax[(v0 / XT + blockIdx.x) * M + m] : 0.f;
+        const float l = m < M ? lse[m] : 0.f;
+        f[threadIdx.x] = m < M ? g * __expf(mx == -__builtin_inff() ? -__builtin_inff() : mx - l) : 0.f;
+        const long long lab = m < M ? labels[m] - v0 - n0 : -1;
+        own[threadIdx.x] = lab >= 0 && lab < XT ? (int)lab : -1;
+        at_label[threadIdx.x] = own[threadIdx.x] >= 0 && g != 0.f ? g * expm1f(zlab[m] - l) : 0.f;
+    }
+    __syncthreads();
+    const int cl = (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < 8; ++i) {
+        const int r = rl + i * 8;
+        const long long m = m0 + r;
+        if (m >= M) continue;
+        float d[8];
+        if (PL == 1) {
+            const s16x8 e = *reinterpret_cast<const s16x8*>(static_cast<const short*>(E) + m * lde + e0 + n0 + cl);
 #pragma unroll
-    for (int a = 0; a < 4; ++a)
+            for (int j = 0; j < 8; ++j) d[j] = __uint_as_float((unsigned)(unsigned short)e[j] << 16);
+        } else {
+            const float* p = static_cast<const float*>(E) + m * lde + e0 + n0 + cl;
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const long long k = k0 + ty + 16 * a, n = n0 + tx + 16 * c;
-            if (k < K && n < cols) xe_store(DW + k * V + v0 + n, acc[a][c]);
+            for (int j = 0; j < 4; ++j) {
+                d[j] = a[j];
+                d[4 + j] = b[j];
+            }
         }
+        s16x8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = cl + j == own[r] ? at_label[r] : d[j] * f[r];
+            sum[j] += v;
+            if (PL == 1) {
+                hi[j] = xe_bf16(v);
+            } else {
+                const float s = v * XE_DZ_SCALE;
+                const _Float16 h = (_Float16)s;
+                hi[j] = __builtin_bit_cast(short, h);
+                lo[j] = __builtin_bit_cast(short, (_Float16)(s - (float)h));
+            }
+        }
+        short* out = dz + m * ld + (PL == 1 ? n0 + cl : (n0 + cl) / 32 * 64 + cl % 32);
+        *reinterpret_cast<s16x8*>(out) = hi;
+        if (PL == 2) *reinterpret_cast<s16x8*>(out + 32) = lo;
+    }
+    if (!dbp) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sums[rl][cl + j] = sum[j];
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += sums[k][threadIdx.x];
+    dbp[(long long)blockIdx.y * (ld / PL) + n0 + threadIdx.x] = s;
 }
 
+__device__ __forceinline__ void xe_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void xe_put(__hip_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+
 template <typename T>
-__global__ __launch_bounds__(256) void xe_db_kernel(const float* __restrict__ dz, long long ld, long long M, long long cols,
-                                                    T* __restrict__ DB) {
+__global__ __launch_bounds__(256) void xe_db_kernel(const float* __restrict__ dbp, long long blocks, long long ld, long long cols,
+                                                    const float* __restrict__ scale, T* __restrict__ DB) {
     const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
     if (n >= cols) return;
-    float s = 0.f;
-    for (long long m = 0; m < M; ++m) s += dz[m * ld + n];
-    xe_store(DB + n, s);
+    double s = 0.0;
+    for (long long r = 0; r < blocks; ++r) s += (double)dbp[r * ld + n];
+    xe_put(DB + n, (float)s * *scale);
 }
 
-long long xe_piece(long long M, long long V) {
-    long long p = (64ll << 20) / (M * 4) / XT * XT;
-    if (p < XT) p = XT;
-    const long long all = (V + XT - 1) / XT * XT;
-    return p < all ? p : all;
+// ---- slab [split][M][ldk] (+)= dz w^T over a range of the piece's classes
+template <int PL, int LN, int WL, int WR>
+__global__ __launch_bounds__(64 * WL * WR) void xe_dx_kernel(const short* __restrict__ dz, long long ldz, const short* __restrict__ W,
+                                                             long long ldw, long long w_left, long long M, long long K, int blocks,
+                                                             int splits, int accumulate, float* __restrict__ slab, long long ldk) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false> G;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const long long nrow = (M + LN - 1) / LN, ncol = (K + XT - 1) / XT, tiles = nrow * ncol;
+    const int split = (int)(blockIdx.x / tiles);
+    long long rt, ct;
+    xe_tile_of(blockIdx.x - split * tiles, tiles, nrow, ncol, rt, ct);
+    const int b0 = (int)((long long)blocks * split / splits), b1 = (int)((long long)blocks * (split + 1) / splits);
+    const long long m0 = rt * LN, k0 = ct * XT, skip = (long long)b0 * 128;
+    const Tile tl = {reinterpret_cast<const char*>(dz + m0 * ldz) + skip, (M - m0) * ldz * 2 - skip, ldz * 2};
+    const Tile tr = {reinterpret_cast<const char*>(W + k0 * ldw) + skip, w_left - k0 * ldw * 2 - skip, ldw * 2};
+    f32x16 acc[G::TL][G::TR];
+    G::run(tl, tr, b1 - b0, (lds_char*)smem, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
+#pragma unroll
+    for (int a = 0; a < G::TL; ++a) {
+        const long long m = m0 + wl * (LN / WL) + a * 32 + (lane & 31);
+        if (m >= M) continue;
+#pragma unroll
+        for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const long long k = k0 + wr * (XT / WR) + b * 32 + q * 8 + 4 * (lane >> 5);
+                if (k >= ldk) continue;
+                float* out = slab + ((long long)split * M + m) * ldk + k;
+                f32x4 v = {acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
+                if (accumulate) v += *reinterpret_cast<const f32x4*>(out);
+                *reinterpret_cast<f32x4*>(out) = v;
+            }
+    }
 }
 
-template <typename T>
-int xe_forward(const void* X, const void* W, const void* Bv, const long long* labels, long long M, long long K, long long V, int bf16,
-               long long ignore, float* loss, float* lse, float* zlab, float* totals, float* ws, hipStream_t stream) {
-    const long long nt = (V + XT - 1) / XT;
-    hipLaunchKernelGGL((xe_logits_kernel<T, false>), dim3((unsigned)nt, (unsigned)((M + XT - 1) / XT)), dim3(256), 0, stream,
-                       static_cast<const T*>(X), static_cast<const T*>(W), static_cast<const T*>(Bv), labels, M, K, V, 0ll, V, bf16,
-                       ignore, ws, ws + M * nt, nt, zlab, nullptr, nullptr, 0, nullptr, 0, nullptr, 0ll);
-    DTF_CHECK_LAUNCH();
-    hipLaunchKernelGGL(xe_merge_kernel, dim3((unsigned)M), dim3(64), 0, stream, ws, ws + M * nt, nt, labels, V, ignore, zlab, lse,
-                       loss);
-    DTF_CHECK_LAUNCH();
-    hipLaunchKernelGGL(xe_total_kernel, dim3(1), dim3(256), 0, stream, loss, labels, M, ignore, totals);
+template <typename T, int PL>
+__global__ __launch_bounds__(256) void xe_dx_finish_kernel(const float* __restrict__ slab, int splits, long long M, long long K,
+                                                           long long ldk, const unsigned* __restrict__ amax,
+                                                           const float* __restrict__ scale, T* __restrict__ DX) {
+    const float iw = PL == 2 ? 1.f / xe_scale(amax[1]) / XE_DZ_SCALE : 1.f;
+    const float g = *scale;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < M * K; i += (long long)gridDim.x * 256) {
+        const long long m = i / K, k = i - m * K;
+        float s = 0.f;
+        for (int p = 0; p < splits; ++p) s += slab[((long long)p * M + m) * ldk + k];
+        xe_put(DX + i, s * iw * g);
+    }
+}
+
+// ---- dw[:, v0 ...] = x^T dz
+template <int PL, int OUT_BF16>
+__global__ __launch_bounds__(512) void xe_dw_kernel(const short* __restrict__ X, long long ldx, const short* __restrict__ dz, long long ldz,
+                                                    long long M, long long K, long long cols, const unsigned* __restrict__ amax,
+                                                    const float* __restrict__ scale, void* __restrict__ DW, long long V, long long v0) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, 256, XT, 2, 4, true, true> G;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const long long nrow = (K + 255) / 256, ncol = (cols + XT - 1) / XT;
+    long long rt, ct;
+    xe_tile_of(blockIdx.x, nrow * ncol, nrow, ncol, rt, ct);
+    const long long k0 = rt * 256, n0 = ct * XT;
+    const Tile tl = {reinterpret_cast<const char*>(X + k0 * PL), M * ldx * 2 - k0 * PL * 2, ldx * 2};
+    const Tile tr = {reinterpret_cast<const char*>(dz + n0 * PL), M * ldz * 2 - n0 * PL * 2, ldz * 2};
+    f32x16 acc[G::TL][G::TR];
+    G::run(tl, tr, (int)((M + G::CB - 1) / G::CB), (lds_char*)smem, acc);
+    const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) / XE_DZ_SCALE : 1.f;
+    const float g = *scale;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / 4, wr = wave % 4;
+#pragma unroll
+    for (int a = 0; a < G::TL; ++a) {
+        const long long k = k0 + wl * 128 + a * 32 + (lane & 31);
+        if (OUT_BF16) {
+            short* out = static_cast<short*>(DW) + k * V + v0;
+            const long long n = n0 + wr * 64 + 8 * (lane >> 5);
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b) {
+                if (n0 + wr * 64 + b * 32 + 32 <= cols) {
+                    hgemm::store_bf16_16(acc[a][b], g, out + n + b * 32, k < K);
+                } else if (k < K) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const long long c = n0 + wr * 64 + b * 32 + (r >> 2) * 8 + 4 * (lane >> 5) + (r & 3);
+                        if (c < cols) out[c] = xe_bf16(acc[a][b][r] * g);
+                    }
+                }
+            }
+        } else {
+            float* out = static_cast<float*>(DW) + k * V + v0;
+            if (k >= K) continue;
+#pragma unroll
+            for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const long long c = n0 + wr * 64 + b * 32 + q * 8 + 4 * (lane >> 5);
+                    hgemm::f32x4_any v;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = acc[a][b][q * 4 + i] * ix * g;
+                    if (c + 4 <= cols) {
+                        *reinterpret_cast<hgemm::f32x4_any*>(out + c) = v;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (c + i < cols) out[c + i] = v[i];
+                    }
+                }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+inline long long up(long long v, long long to) { return (v + to - 1) / to * to; }
+inline long long lowest(long long a, long long b) { return a < b ? a : b; }
+
+struct Plan {
+    long long M, K, V;
+    int type, pl;              // 0 fp32, 1 bf16 operands; limbs a value
+    bool packs;                // w has to be packed
+    bool small;                // 64 rows a tile
+    long long ldx, ldw, piece, tiles;
+    long long esize;
+    int splits;                // of the classes of a piece for dx
+    long long ldk;
+};
+
+Plan make_plan(const void* W, long long M, long long K, long long V, int type, int bf16) {
+    Plan p;
+    p.M = M, p.K = K, p.V = V, p.type = type;
+    p.pl = type == 0 && !bf16 ? 2 : 1;
+    const int cb = 64 / p.pl;
+    p.packs = type == 0 || V % 8 != 0 || (reinterpret_cast<uintptr_t>(W) & 15) != 0;
+    // 64 rows a tile while they waste less of the matrix instructions than they read w more often
+    p.small = M <= 128;
+    p.ldx = up(K, cb) * p.pl;
+    p.tiles = (V + XT - 1) / XT;
+    p.esize = p.pl == 2 ? 4 : 2;
+    long long piece = XE_PIECE_BYTES / (M * 2 * p.pl);
+    if (p.packs) piece = lowest(piece, XE_PACK_BYTES / (K * 2 * p.pl));
+    piece = piece / XT * XT;
+    if (piece < XT) piece = XT;
+    p.piece = lowest(piece, p.tiles * XT);
+    p.ldw = p.packs ? p.piece * p.pl : V;
+    // enough workgroups for the chip from a product with few output tiles: the reduction over classes is split, eight stages
+    // at least a split
+    const long long out = ((M + (p.small ? 63 : 255)) / (p.small ? 64 : 256)) * ((K + XT - 1) / XT);
+    const long long blocks = p.piece / cb;
+    p.splits = (int)lowest(lowest((256 + out - 1) / out, blocks / 8 > 0 ? blocks / 8 : 1), 64);
+    p.ldk = up(K, 4);
+    return p;
+}
+
+struct Carver {
+    char* base;
+    long long used = 0;
+    explicit Carver(void* p) : base(static_cast<char*>(p)) {}
+    template <typename T>
+    T* take(long long n) {
+        T* r = reinterpret_cast<T*>(base + used);
+        used += up(n * (long long)sizeof(T), 256);
+        return r;
+    }
+};
+
+struct FwdBuffers {
+    short *x, *w;
+    float *tsum, *beaten, *hit;
+    long long bytes;
+    FwdBuffers(const Plan& p, void* ws) {
+        Carver c(ws);
+        x = c.take<short>(p.M * p.ldx);
+        w = c.take<short>(p.packs ? p.K * p.ldw : 0);
+        tsum = c.take<float>(p.M * p.tiles);
+        beaten = c.take<float>(p.M);
+        hit = c.take<float>(p.M);
+        bytes = c.used;
+    }
+};
+
+struct BwdBuffers {
+    short *x, *w, *dz;
+    void* e;
+    float *slab, *rowg, *scale, *dbp;
+    BwdBuffers(const Plan& p, void* ws) {
+        Carver c(ws);
+        x = c.take<short>(p.M * p.ldx);
+        w = c.take<short>(p.packs ? p.K * p.ldw : 0);
+        dz = c.take<short>(p.M * p.piece * p.pl);
+        e = c.take<char>(p.M * p.piece * p.esize);
+        slab = c.take<float>(p.splits * p.M * p.ldk);
+        rowg = c.take<float>(p.M);
+        scale = c.take<float>(1);
+        dbp = c.take<float>((p.M + 63) / 64 * p.piece);
+        bytes = c.used;
+    }
+    long long bytes;
+};
+
+template <typename F>
+int with_lds(F* kernel, int bytes) {
+    return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+#define XE_TRY(call)              \
+    do {                          \
+        const int rc__ = (call);  \
+        if (rc__ != 0) return rc__; \
+    } while (0)
+
+int pack(const Plan& p, const void* src, long long ld_src, long long rows, long long cols, short* dst, long long ld,
+         const long long* labels, long long ignore, const unsigned* amax, hipStream_t stream) {
+    const long long total = rows * (ld / p.pl / 8);
+    const unsigned grid = (unsigned)lowest((total + 255) / 256, 8192);
+    const int align = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld_src % (p.type ? 8 : 4) == 0;
+    if (p.type == 1)
+        hipLaunchKernelGGL((xe_pack_kernel<__hip_bfloat16, 1>), dim3(grid), dim3(256), 0, stream,
+                           static_cast<const __hip_bfloat16*>(src), ld_src, rows, cols, dst, ld, labels, ignore, amax, align);
+    else if (p.pl == 1)
+        hipLaunchKernelGGL((xe_pack_kernel<float, 1>), dim3(grid), dim3(256), 0, stream, static_cast<const float*>(src), ld_src, rows,
+                           cols, dst, ld, labels, ignore, amax, align);
+    else
+        hipLaunchKernelGGL((xe_pack_kernel<float, 2>), dim3(grid), dim3(256), 0, stream, static_cast<const float*>(src), ld_src, rows,
+                           cols, dst, ld, labels, ignore, amax, align);
     DTF_CHECK_LAUNCH();
     return 0;
 }
 
-template <typename T>
-int xe_backward(const void* X, const void* W, const void* Bv, const long long* labels, long long M, long long K, long long V, int bf16,
-                long long ignore, const float* lse, const float* totals, int mean, const float* dloss, int dloss_stride, void* DX,
-                void* DW, void* DB, float* ws, hipStream_t stream) {
-    const long long piece = xe_piece(M, V);
-    float* dz = ws;
-    float* dx32 = ws + M * piece;
-    const T *x = static_cast<const T*>(X), *w = static_cast<const T*>(W), *b = static_cast<const T*>(Bv);
-    const unsigned mt = (unsigned)((M + XT - 1) / XT), kt = (unsigned)((K + XT - 1) / XT);
-    for (long long v0 = 0; v0 < V; v0 += piece) {
-        const long long cols = v0 + piece < V ? piece : V - v0;
-        const unsigned nt = (unsigned)((cols + XT - 1) / XT);
-        hipLaunchKernelGGL((xe_logits_kernel<T, true>), dim3(nt, mt), dim3(256), 0, stream, x, w, b, labels, M, K, V, v0, v0 + cols,
-                           bf16, ignore, nullptr, nullptr, 0ll, nullptr, lse, dloss, dloss_stride, totals, mean, dz, piece);
+// w of the classes [v0, v0 + cols): packed into `buf`, or in place.  *left: bytes from there to the end of the operand.
+int piece_of_w(const Plan& p, const void* W, long long v0, long long cols, short* buf, const unsigned* amax, hipStream_t stream,
+               const short** w, long long* left) {
+    const char* src = static_cast<const char*>(W) + v0 * (p.type ? 2 : 4);
+    if (!p.packs) {
+        *w = reinterpret_cast<const short*>(src);
+        *left = (p.K * p.V - v0) * 2;
+        return 0;
+    }
+    *w = buf;
+    *left = p.K * p.ldw * 2;
+    return pack(p, src, p.V, p.K, cols, buf, p.ldw, nullptr, 0, amax + 1, stream);
+}
+
+struct Call {
+    const void *X, *W, *B;
+    const long long* labels;
+    long long ignore;
+    hipStream_t stream;
+};
+
+template <int PL, int LN, int WL, int WR>
+int launch_logits(const Plan& p, const Call& c, const short* x, const short* w, long long left, long long v0, long long vend,
+                  const unsigned* amax, float* tmax, float* tsum, float* zlab, float* beaten, void* E, long long lde, long long e0,
+                  long long e_tiles) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
+    auto* kernel = &xe_logits_kernel<PL, LN, WL, WR>;
+    XE_TRY(with_lds(kernel, G::LDS_BYTES));
+    const long long tiles = ((p.M + LN - 1) / LN) * ((vend - v0 + XT - 1) / XT);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(G::THREADS), G::LDS_BYTES, c.stream, x, p.ldx, w, p.ldw, left, c.B,
+                       p.type, c.labels, p.M, p.K, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+int logits(const Plan& p, const Call& c, const short* x, const short* w, long long left, long long v0, long long vend,
+           const unsigned* amax, float* tmax, float* tsum, float* zlab, float* beaten, void* E, long long lde, long long e0,
+           long long e_tiles) {
+    if (p.pl == 1)
+        return p.small ? launch_logits<1, 64, 1, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles)
+                       : launch_logits<1, 256, 2, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
+    return p.small ? launch_logits<2, 64, 1, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles)
+                   : launch_logits<2, 256, 2, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
+}
+
+template <int PL, int LN, int WL, int WR>
+int launch_dx(const Plan& p, const short* dz, const short* w, long long left, long long cols, int first, float* slab, hipStream_t stream) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false> G;
+    auto* kernel = &xe_dx_kernel<PL, LN, WL, WR>;
+    XE_TRY(with_lds(kernel, G::LDS_BYTES));
+    const long long tiles = ((p.M + LN - 1) / LN) * ((p.K + XT - 1) / XT);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.splits)), dim3(G::THREADS), G::LDS_BYTES, stream, dz, p.piece * PL, w, p.ldw,
+                       left, p.M, p.K, (int)((cols + G::CB - 1) / G::CB), p.splits, !first, slab, p.ldk);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+template <int PL, int OUT_BF16>
+int launch_dw(const Plan& p, const short* x, const short* dz, long long v0, long long cols, const unsigned* amax, const float* scale,
+              void* DW, hipStream_t stream) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, 256, XT, 2, 4, true, true> G;
+    auto* kernel = &xe_dw_kernel<PL, OUT_BF16>;
+    XE_TRY(with_lds(kernel, G::LDS_BYTES));
+    const long long tiles = ((p.K + 255) / 256) * ((cols + XT - 1) / XT);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
+                       cols, amax, scale, DW, p.V, v0);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, float* tmax, float* totals, unsigned* amax, void* kept,
+            long long kept_cols, void* ws) {
+    const FwdBuffers b(p, ws);
+    if (p.pl == 2) {
+        hipLaunchKernelGGL(xe_zero_kernel, dim3(1), dim3(2), 0, c.stream, amax);
         DTF_CHECK_LAUNCH();
-        if (DX) {
-            hipLaunchKernelGGL(xe_dx_kernel<T>, dim3(kt, mt), dim3(256), 0, stream, dz, piece, w, M, K, V, v0, cols, bf16, v0 == 0,
-                               v0 + piece >= V, dx32, static_cast<T*>(DX));
+        hipLaunchKernelGGL(xe_amax_kernel, dim3(1024, 2), dim3(256), 0, c.stream, static_cast<const float*>(c.X), p.M, p.K, c.labels,
+                           c.ignore, static_cast<const float*>(c.W), p.K * p.V, amax);
+        DTF_CHECK_LAUNCH();
+    }
+    XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, amax, c.stream));
+    // where w is read in place the whole vocabulary is one launch (bounded by the grid: 4194304 tiles)
+    const long long rowtiles = (p.M + (p.small ? 63 : 255)) / (p.small ? 64 : 256);
+    const long long step = p.packs ? p.piece : lowest(p.V, (1 << 22) / rowtiles * XT);
+    for (long long v0 = 0; v0 < p.V; v0 += step) {
+        const long long cols = lowest(step, p.V - v0);
+        const short* w;
+        long long left;
+        XE_TRY(piece_of_w(p, c.W, v0, cols, b.w, amax, c.stream, &w, &left));
+        const long long e_tiles = kept_cols > v0 ? (kept_cols - v0) / XT : 0;
+        XE_TRY(logits(p, c, b.x, w, left, v0, v0 + cols, amax, tmax, b.tsum, zlab, b.beaten, kept, kept_cols, v0, e_tiles));
+    }
+    int rows = 64;
+    while (rows > 1 && rows / 2 >= p.M) rows /= 2;
+    hipLaunchKernelGGL(xe_merge_kernel, dim3((unsigned)((p.M + rows - 1) / rows)), dim3(256), 0, c.stream, tmax, b.tsum, p.tiles,
+                       c.labels, p.M, p.V, c.ignore, rows, zlab, b.beaten, lse, loss, b.hit);
+    DTF_CHECK_LAUNCH();
+    hipLaunchKernelGGL(xe_total_kernel, dim3(1), dim3(1024), 0, c.stream, loss, b.hit, c.labels, p.M, c.ignore, totals);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, float* tmax, const float* totals, const unsigned* amax,
+             const void* kept, long long kept_cols, int mean, const float* dloss, int stride, void* DX, void* DW, void* DB, void* ws) {
+    const BwdBuffers b(p, ws);
+    hipLaunchKernelGGL(xe_weights_kernel, dim3(1), dim3(1024), 0, c.stream, dloss, stride, totals, mean, c.labels, p.M, p.V, c.ignore,
+                       lse, zlab, b.rowg, b.scale);
+    DTF_CHECK_LAUNCH();
+    if (DW || kept_cols < p.V) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, amax, c.stream));
+    const long long rowblocks = (p.M + 63) / 64;
+    for (long long v0 = 0; v0 < p.V; v0 += p.piece) {
+        const long long cols = lowest(p.piece, p.V - v0), ct = (cols + XT - 1) / XT;
+        const short* w = nullptr;
+        long long left = 0;
+        const long long have = kept_cols > v0 ? lowest((kept_cols - v0) / XT, ct) : 0;      // the piece's tiles whose e was kept
+        if (DX || have < ct) XE_TRY(piece_of_w(p, c.W, v0, cols, b.w, amax, c.stream, &w, &left));
+        float* dbp = DB ? b.dbp : nullptr;
+        for (int part = 0; part < 2; ++part) {
+            const long long t0 = part ? have : 0, t1 = part ? ct : have, at = v0 + t0 * XT;
+            if (t1 == t0) continue;
+            const void* e = kept;
+            long long lde = kept_cols, e0 = at;
+            if (part) {      // not kept: computed again
+                e = b.e, lde = p.piece, e0 = t0 * XT;
+                XE_TRY(logits(p, c, b.x, w + t0 * XT * p.pl, left - t0 * XT * p.pl * 2, at, v0 + cols, amax, nullptr, nullptr, nullptr,
+                              nullptr, b.e, p.piece, e0, t1 - t0));
+            }
+            short* dz = b.dz + t0 * XT * p.pl;
+            float* sums = dbp ? dbp + t0 * XT : nullptr;
+            const dim3 grid((unsigned)(t1 - t0), (unsigned)rowblocks);
+            if (p.pl == 1)
+                hipLaunchKernelGGL(xe_dz_kernel<1>, grid, dim3(256), 0, c.stream, e, lde, e0, tmax, lse, zlab, b.rowg, c.labels, p.M, at,
+                                   dz, p.piece, sums);
+            else
+                hipLaunchKernelGGL(xe_dz_kernel<2>, grid, dim3(256), 0, c.stream, e, lde, e0, tmax, lse, zlab, b.rowg, c.labels, p.M, at,
+                                   dz, p.piece * 2, sums);
             DTF_CHECK_LAUNCH();
+        }
+        if (DX) {
+            const int first = v0 == 0;
+            if (p.pl == 1)
+                XE_TRY(p.small ? (launch_dx<1, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
+                               : (launch_dx<1, 256, 2, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream)));
+            else
+                XE_TRY(p.small ? (launch_dx<2, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
+                               : (launch_dx<2, 256, 2, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream)));
         }
         if (DW) {
-            hipLaunchKernelGGL(xe_dw_kernel<T>, dim3(nt, kt), dim3(256), 0, stream, x, dz, piece, labels, M, K, V, v0, cols, bf16,
-                               ignore, static_cast<T*>(DW));
-            DTF_CHECK_LAUNCH();
+            if (p.pl == 2) XE_TRY((launch_dw<2, 0>(p, b.x, b.dz, v0, cols, amax, b.scale, DW, c.stream)));
+            else if (p.type == 1) XE_TRY((launch_dw<1, 1>(p, b.x, b.dz, v0, cols, amax, b.scale, DW, c.stream)));
+            else XE_TRY((launch_dw<1, 0>(p, b.x, b.dz, v0, cols, amax, b.scale, DW, c.stream)));
         }
         if (DB) {
-            hipLaunchKernelGGL(xe_db_kernel<T>, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, stream, dz, piece, M, cols,
-                               static_cast<T*>(DB) + v0);
+            const dim3 grid((unsigned)((cols + 255) / 256));
+            if (p.type == 1)
+                hipLaunchKernelGGL(xe_db_kernel<__hip_bfloat16>, grid, dim3(256), 0, c.stream, b.dbp, rowblocks, p.piece, cols, b.scale,
+                                   static_cast<__hip_bfloat16*>(DB) + v0);
+            else
+                hipLaunchKernelGGL(xe_db_kernel<float>, grid, dim3(256), 0, c.stream, b.dbp, rowblocks, p.piece, cols, b.scale,
+                                   static_cast<float*>(DB) + v0);
             DTF_CHECK_LAUNCH();
         }
+    }
+    if (DX) {
+        const dim3 grid((unsigned)lowest((p.M * p.K + 255) / 256, 16384));
+        if (p.pl == 2)
+            hipLaunchKernelGGL((xe_dx_finish_kernel<float, 2>), grid, dim3(256), 0, c.stream, b.slab, p.splits, p.M, p.K, p.ldk, amax,
+                               b.scale, static_cast<float*>(DX));
+        else if (p.type == 1)
+            hipLaunchKernelGGL((xe_dx_finish_kernel<__hip_bfloat16, 1>), grid, dim3(256), 0, c.stream, b.slab, p.splits, p.M, p.K, p.ldk,
+                               amax, b.scale, static_cast<__hip_bfloat16*>(DX));
+        else
+            hipLaunchKernelGGL((xe_dx_finish_kernel<float, 1>), grid, dim3(256), 0, c.stream, b.slab, p.splits, p.M, p.K, p.ldk, amax,
+                               b.scale, static_cast<float*>(DX));
+        DTF_CHECK_LAUNCH();
     }
     return 0;
 }
 
-bool xe_ok(long long M, long long K, long long V, int type) {
-    return M > 0 && K > 0 && V > 0 && (type == 0 || type == 1) && (M + XT - 1) / XT <= 65535 && (K + XT - 1) / XT <= 65535 &&
-           V <= (1ll << 30) && M <= (1ll << 24);
+bool sizes_ok(long long M, long long K, long long V, int type) {
+    return M > 0 && K > 0 && V > 0 && (type == 0 || type == 1) && M <= 65535ll * 64 && K <= (1ll << 20) && V <= (1ll << 22);
 }
 
 }  // namespace
 
-DTF_API long long dtf_linear_xent_fwd_workspace_bytes(long long M, long long K, long long V, int type, int bf16) {
-    return M * ((V + XT - 1) / XT) * 8;
+// The largest sizes: 4194240 rows, 1048576 features, 4194304 classes (32-bit offsets within a tile; rows in blocks of 64 as
+// the second grid dimension).
+DTF_API int dtf_linear_xent_supported(long long M, long long K, long long V) { return sizes_ok(M, K, V, 0) ? 1 : 0; }
+
+DTF_API long long dtf_linear_xent_fwd_workspace_bytes(const void* W, long long M, long long K, long long V, int type, int bf16) {
+    return sizes_ok(M, K, V, type) ? FwdBuffers(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;
 }
-DTF_API long long dtf_linear_xent_bwd_workspace_bytes(long long M, long long K, long long V, int type, int bf16) {
-    return (M * xe_piece(M, V) + M * K) * 4;
+DTF_API long long dtf_linear_xent_bwd_workspace_bytes(const void* W, long long M, long long K, long long V, int type, int bf16) {
+    return sizes_ok(M, K, V, type) ? BwdBuffers(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;
 }
 
 // type: 0 fp32, 1 bf16 (x, w, b alike; b may be null).  bf16 != 0: fp32 operands rounded to bf16 for the products.
-// loss, lse, zlab: M floats each; totals: 4 floats (sum, counted rows, mean).
+// loss, lse, zlab: M floats each; tmax: M floats for every 256 classes; totals: 4 floats (sum, counted rows, mean, rows whose
+// label has the largest logit); amax: 2 words (fp32 products only).  kept (may be null): [M, kept_cols] fp32 - bf16 where the
+// products take bf16 -, kept_cols a multiple of 256.
 DTF_API int dtf_linear_xent_fwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
-                                long long V, int type, int bf16, long long ignore, float* loss, float* lse, float* zlab,
-                                float* totals, void* workspace, hipStream_t stream) {
-    if (!xe_ok(M, K, V, type)) return -1;
-    float* ws = static_cast<float*>(workspace);
-    if (type == 0) return xe_forward<float>(X, W, B, labels, M, K, V, bf16, ignore, loss, lse, zlab, totals, ws, stream);
-    return xe_forward<__hip_bfloat16>(X, W, B, labels, M, K, V, 1, ignore, loss, lse, zlab, totals, ws, stream);
+                                long long V, int type, int bf16, long long ignore, float* loss, float* lse, float* zlab, float* tmax,
+                                float* totals, unsigned* amax, void* kept, long long kept_cols, void* workspace, hipStream_t stream) {
+    if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
+    const Call c = {X, W, B, labels, ignore, stream};
+    return forward(make_plan(W, M, K, V, type, bf16), c, loss, lse, zlab, tmax, totals, amax, kept, kept ? kept_cols : 0, workspace);
 }
 
 // dloss: the loss's gradient, one float for all rows (stride 0) or one a row (stride 1); mean != 0: divided by the counted
 // rows.  DX, DW, DB may each be null.
 DTF_API int dtf_linear_xent_bwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
-                                long long V, int type, int bf16, long long ignore, const float* lse, const float* zlab,
-                                const float* totals, int mean, const float* dloss, int dloss_stride, void* DX, void* DW, void* DB,
-                                void* workspace, hipStream_t stream) {
-    if (!xe_ok(M, K, V, type)) return -1;
-    float* ws = static_cast<float*>(workspace);
-    if (type == 0)
-        return xe_backward<float>(X, W, B, labels, M, K, V, bf16, ignore, lse, totals, mean, dloss, dloss_stride, DX, DW, DB, ws, stream);
-    return xe_backward<__hip_bfloat16>(X, W, B, labels, M, K, V, 1, ignore, lse, totals, mean, dloss, dloss_stride, DX, DW, DB, ws,
-                                       stream);
+                                long long V, int type, int bf16, long long ignore, const float* lse, const float* zlab, float* tmax,
+                                const float* totals, const unsigned* amax, const void* kept, long long kept_cols, int mean,
+                                const float* dloss, int dloss_stride, void* DX, void* DW, void* DB, void* workspace,
+                                hipStream_t stream) {
+    if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
+    const Call c = {X, W, B, labels, ignore, stream};
+    return backward(make_plan(W, M, K, V, type, bf16), c, lse, zlab, tmax, totals, amax, kept, kept ? kept_cols : 0, mean, dloss,
+                    dloss_stride, DX, DW, DB, workspace);
 }

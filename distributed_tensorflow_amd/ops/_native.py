@@ -90,9 +90,9 @@ def kernels():
         "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, c_f, c_p, c_p, c_p],
         "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p],
         "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
-        "dtf_linear_xent_fwd": [c_p, c_p, c_p, c_p, c_ll, c_ll, c_ll, c_i, c_i, c_ll, c_p, c_p, c_p, c_p, c_p, c_p],
-        "dtf_linear_xent_bwd": [c_p, c_p, c_p, c_p, c_ll, c_ll, c_ll, c_i, c_i, c_ll, c_p, c_p, c_p, c_i, c_p, c_i, c_p, c_p,
-                                c_p, c_p, c_p],
+        "dtf_linear_xent_supported": [c_ll] * 3,
+        "dtf_linear_xent_fwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 7 + [c_ll, c_p, c_p],
+        "dtf_linear_xent_bwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 6 + [c_ll, c_i, c_p, c_i] + [c_p] * 5,
         "dtf_im2col": [c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_col2im": [c_p, c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_avgpool_fwd": [c_p, c_p] + [c_i] * 12 + [c_p],
@@ -126,8 +126,8 @@ def kernels():
             fn.argtypes = argtypes
             fn.restype = c_i
     for name, argtypes in {"dtf_groupnorm_workspace_floats": [c_ll, c_ll, c_i, c_i],
-                           "dtf_linear_xent_fwd_workspace_bytes": [c_ll, c_ll, c_ll, c_i, c_i],
-                           "dtf_linear_xent_bwd_workspace_bytes": [c_ll, c_ll, c_ll, c_i, c_i]}.items():
+                           "dtf_linear_xent_fwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i],
+                           "dtf_linear_xent_bwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i]}.items():
         declare(lib, name, argtypes, c_ll)
     if hasattr(lib, "dtf_batchnorm_workspace_floats"):
         lib.dtf_batchnorm_workspace_floats.argtypes = [c_ll, c_i]

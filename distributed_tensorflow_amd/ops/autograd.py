@@ -135,12 +135,12 @@ def softmax_cross_entropy(logits, labels):
 
 
 class _LinearXentFn(torch.autograd.Function):
-    """Softmax cross-entropy of ``x @ w + b`` without the logits in memory; the backward pass is computed when it is asked
-    for, from the rows' logsumexp."""
+    """Softmax cross-entropy of ``x @ w + b`` without the logits in memory; the gradients are computed when they are asked
+    for."""
 
     @staticmethod
     def forward(ctx, x, w, b, labels, ignore_index, reduction, bf16):
-        loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16)
+        loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16, keep=any(ctx.needs_input_grad[:3]))
         ctx.save_for_backward(x, w, b, labels, *state)
         ctx.cfg = (ignore_index, reduction, bf16)
         if reduction == "none":

@@ -572,8 +572,12 @@ def softmax_xent(z, labels, grad_out=None, grad_scale=None, stats=None):
 
 # --------------------------------------------------------------------------- softmax cross-entropy over a large vocabulary
 _XENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
-#: what ``linear_xent_forward`` keeps for ``linear_xent_backward``; ``totals``: sum of the losses, counted rows, their mean
-LinearXentState = collections.namedtuple("LinearXentState", ["lse", "label_logit", "totals"])
+#: what ``linear_xent_forward`` leaves for ``linear_xent_backward``.  ``totals``: sum of the losses, counted rows, their mean,
+#: rows whose label has the largest logit (ties go to the lowest class); ``kept``: exponentials of the first logits or None
+LinearXentState = collections.namedtuple("LinearXentState", ["lse", "label_logit", "totals", "tile_max", "scales", "kept"])
+#: bytes of exponentials that a forward pass with ``keep=True`` may leave for its backward pass (1/288 of an MI355X's memory)
+LINEAR_XENT_KEEP_BYTES = 1 << 30
+_XENT_TILE = 256
 
 
 def _linear_xent_check(x, w, b, labels):
@@ -589,6 +593,8 @@ def _linear_xent_check(x, w, b, labels):
     for t in (x, w, b, labels):
         if t is not None and (t.device != x.device or not t.is_contiguous()):
             raise ValueError("x, w, b and labels must be contiguous and on one device")
+    if x.shape[0] > 4194240 or x.shape[1] > (1 << 20) or w.shape[1] > (1 << 22):
+        raise ValueError("at most 4194240 rows, 1048576 features and 4194304 classes, got %s, %s" % (tuple(x.shape), tuple(w.shape)))
 
 
 def _linear_xent_logits(x, w, b, labels, ignore_index, bf16):
@@ -602,28 +608,38 @@ def _linear_xent_logits(x, w, b, labels, ignore_index, bf16):
     return x32, w32, z if b is None else z + b.float(), counted
 
 
-def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False):
+def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False):
     """Softmax cross-entropy of the logits ``x @ w + b`` (x [M, K], w [K, V], b [V] or None; all float32 or all bfloat16)
     against int64 ``labels`` [M], for vocabularies whose [M, V] logits should not be in memory.
 
     Rows with the label ``ignore_index`` count for nothing, whatever x holds there; any other label outside ``[0, V)`` makes
     its row's loss NaN.  Classes may be masked by a ``b`` of -infinity.  ``bf16=True``: float32 operands are rounded to
-    bfloat16 for the products.  Returns ``(loss [M] float32, state)``; the state is what ``linear_xent_backward`` needs."""
+    bfloat16 for the products.  Returns ``(loss [M] float32, state)``; the state is what ``linear_xent_backward`` needs.
+
+    ``keep=True`` (a backward pass will follow): up to ``LINEAR_XENT_KEEP_BYTES`` of the first classes' exponentials stay in
+    the state, which saves the backward pass their part of the product; it computes the others again, piece by piece."""
     _linear_xent_check(x, w, b, labels)
     M, K, V = int(x.shape[0]), int(x.shape[1]), int(w.shape[1])
-    new = lambda n: torch.empty(n, dtype=torch.float32, device=x.device)
-    loss, state = new(M), LinearXentState(new(M), new(M), new(4))
+    tiles = -(-V // _XENT_TILE)
+    new = lambda *n: torch.empty(n, dtype=torch.float32, device=x.device)
+    cols = 0
+    if keep and M and x.is_cuda:
+        size = 2 if bf16 or x.dtype == torch.bfloat16 else 4
+        cols = min(tiles, LINEAR_XENT_KEEP_BYTES // (M * size * _XENT_TILE)) * _XENT_TILE
+    kept = torch.empty((M, cols), dtype=torch.bfloat16 if size == 2 else torch.float32, device=x.device) if cols else None
+    loss, state = new(M), LinearXentState(new(M), new(M), new(4), new(tiles, M) if x.is_cuda else None, new(2), kept)
     if M == 0:
         state.totals.zero_()
         return loss, state
     if x.is_cuda:
         with nv.device_guard(x):
             lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
-            ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(M, K, V, t, int(bf16))), dtype=torch.uint8,
-                             device=x.device)
+            ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(nv.ptr(w), M, K, V, t, int(bool(bf16)))),
+                             dtype=torch.uint8, device=x.device)
             rc = lib.dtf_linear_xent_fwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
                                          int(ignore_index), nv.ptr(loss), nv.ptr(state.lse), nv.ptr(state.label_logit),
-                                         nv.ptr(state.totals), nv.ptr(ws), nv.stream_ptr())
+                                         nv.ptr(state.tile_max), nv.ptr(state.totals), nv.ptr(state.scales), nv.ptr(kept), cols,
+                                         nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_fwd")
         return loss, state
     _, _, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
@@ -633,7 +649,8 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False):
     state.label_logit.copy_(torch.where(valid, picked, torch.full_like(picked, float("nan"))))
     loss.copy_(torch.where(counted, state.lse - state.label_logit, torch.zeros_like(loss)))
     n = int(counted.sum())
-    state.totals.copy_(torch.tensor([float(loss.double().sum()), n, float(loss.double().sum()) / max(n, 1), 0.0]))
+    hits = int((counted & valid & (z.argmax(dim=1) == labels)).sum())
+    state.totals.copy_(torch.tensor([float(loss.double().sum()), n, float(loss.double().sum()) / max(n, 1), hits]))
     return loss, state
 
 
@@ -659,12 +676,14 @@ def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index
     if x.is_cuda:
         with nv.device_guard(x):
             lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
-            ws = torch.empty(int(lib.dtf_linear_xent_bwd_workspace_bytes(M, K, V, t, int(bf16))), dtype=torch.uint8,
-                             device=x.device)
+            kept = state.kept
+            ws = torch.empty(int(lib.dtf_linear_xent_bwd_workspace_bytes(nv.ptr(w), M, K, V, t, int(bool(bf16)))),
+                             dtype=torch.uint8, device=x.device)
             rc = lib.dtf_linear_xent_bwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
-                                         int(ignore_index), nv.ptr(state.lse), nv.ptr(state.label_logit), nv.ptr(state.totals),
-                                         int(bool(mean)), nv.ptr(dloss), int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw),
-                                         nv.ptr(db), nv.ptr(ws), nv.stream_ptr())
+                                         int(ignore_index), nv.ptr(state.lse), nv.ptr(state.label_logit),
+                                         nv.ptr(state.tile_max), nv.ptr(state.totals), nv.ptr(state.scales), nv.ptr(kept),
+                                         0 if kept is None else kept.shape[1], int(bool(mean)), nv.ptr(dloss),
+                                         int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw), nv.ptr(db), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_bwd")
         return
     x32, w32, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
