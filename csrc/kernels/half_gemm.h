@@ -9,12 +9,18 @@
 // product): 32 values of a row are stored as 32 hi limbs, then 32 lo limbs, so that a tile of 2-limb values has the shape of
 // a tile of 16-bit values with half as many k.  Three limb products make one product: hi hi, hi lo, lo hi.
 //
-// A workgroup of WL x WR waves computes an LN x RN tile; a wave holds (LN / WL) x (RN / WR) of it in accumulators.  A stage is
+// A workgroup of WL x WR waves computes LN x RN tiles one after another; a wave holds (LN / WL) x (RN / WR) in accumulators.  A stage is
 // 64 halves of the reduction an operand row: 128 bytes a row, loaded straight into LDS (16 bytes a lane); while one stage
 // is multiplied the next one arrives in the other buffer, one barrier a stage.
 //
-// LDS layouts.  RC: row of 128 bytes = 8 chunks of 16; chunk c of row i lies at c ^ (i & 7), so that the 32 rows that a
-// fragment read touches at one c spread over all banks.  RS: row k of LN * PL halves in granules of 32 bytes; granule q of
+// What bounds it (8192 x 8192 x 2048, bf16): power and the loads into LDS.  The matrix pipes are busy 58 % of the cycles at a
+// clock that the load drives down to 1.9 GHz; without the loads in the loop the same instructions reach 1400 TFLOP/s, without
+// LDS reads 1200, without both 1550.  Measured and dropped: a ring of four half stages (64 bytes a row: 1070), 128 x 128 a
+// wave (the compiler spills its accumulators), padded rows (no effect: the strides do not meet in one channel).
+//
+// LDS layouts.  RC: row of 128 bytes = 8 chunks of 16; chunk c of row i lies at c ^ ((i >> 1) & 7): LDS delivers 256 bytes a
+// cycle, 16 lanes of a fragment read, whose 16 rows at one c are then on 16 different chunks of two rows' width (with i & 7
+// every second chunk would be hit twice: measured as one conflict cycle for each useful one).  RS: row k of LN * PL halves in granules of 32 bytes; granule q of
 // row k lies at q ^ 2 (k & 3): a transposing read takes 4 rows x 2 granules at once, which are then 8 distinct ones of 256 bytes.
 // The direct load writes LDS linearly, so the permutation is applied to the addresses it loads from.
 #pragma once
@@ -68,6 +74,13 @@ __device__ __forceinline__ void store_bf16_16(const f32x16& acc, float g, short*
     }
 }
 
+// Transposing read: of every 16 lanes, lane i receives value i of 4 rows, from the 4 lanes that address each row (4 values a lane).
+// __restrict__ gives the read a scope of its own; without one the compiler waits for all loads into LDS that are in flight
+// before it, also for those into the other buffer.  (The waits that are needed are written out in the loop.)
+__device__ __forceinline__ s16x4 read_tr(const lds_char* __restrict__ p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+}
+
 // One operand's tile in memory: `base` is its first element, `left` the bytes from there to the end of the operand (what lies
 // behind reads as zero), `ld` the bytes of a row.
 struct Tile {
@@ -94,31 +107,33 @@ struct Gemm {
     // LDS <- stage `blk` of one operand
     template <int N, bool RS>
     static __device__ __forceinline__ void load(const Tile& t, int blk, lds_char* dst) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));                       // the offsets are worked out anew each stage: kept, they would spill
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         constexpr int LOADS = N / 8 / WAVES;                 // 1 KB each
         if (!RS) {
             const __amdgpu_buffer_rsrc_t rs = resource(t.base + (long long)blk * 128, t.left - (long long)blk * 128);
             const unsigned ld = (unsigned)t.ld;
-            unsigned off = (unsigned)(wave * LOADS * 8 + (lane >> 3)) * ld + (unsigned)(((lane & 7) ^ (lane >> 3)) * 16);
+            static_assert(LOADS % 2 == 0, "the chunk permutation of a load depends on its parity");
+            const unsigned row0 = (unsigned)(wave * LOADS * 8 + (lane >> 3)) * ld;
+            const unsigned chunk = (unsigned)((lane & 7) ^ (lane >> 4)) * 16;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
+            for (int i = 0; i < LOADS; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
-                                                         (int)off, 0, 0, 0);
-                off += 8 * ld;
-            }
+                                                         (int)(row0 + 8 * i * ld + (i & 1 ? chunk ^ 64 : chunk)), 0, 0, 0);
         } else {
             constexpr int SLOTS = N * PL / 8;                // 16-byte chunks a row: 32 or 64
             constexpr int ROWS = 64 / SLOTS;                 // rows a load: 2 or 1
             const long long skip = (long long)blk * CB * t.ld;
             const __amdgpu_buffer_rsrc_t rs = resource(t.base + skip, t.left - skip);
             const unsigned ld = (unsigned)t.ld;
+            static_assert(LOADS * ROWS % 4 == 0, "a wave's first row is a multiple of 4");
+            const unsigned row0 = (unsigned)(wave * LOADS * ROWS + lane / SLOTS) * ld;
+            const unsigned chunk = (unsigned)((lane % SLOTS) ^ (4 * (lane / SLOTS))) * 16;
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int row = (wave * LOADS + i) * ROWS + lane / SLOTS;
-                const int chunk = (lane % SLOTS) ^ (4 * (row & 3));
+            for (int i = 0; i < LOADS; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
-                                                         (int)((unsigned)row * ld + (unsigned)chunk * 16), 0, 0, 0);
-            }
+                                                         (int)(row0 + ROWS * i * ld + (chunk ^ (64 * (ROWS * i & 3)))), 0, 0, 0);
         }
     }
 
@@ -128,65 +143,149 @@ struct Gemm {
         const int lane = threadIdx.x & 63;
         if (!RS) {
             const int chunk = plane * 4 + kk * 2 + (lane >> 5);
-            return *(const __attribute__((address_space(3))) s16x8*)(src + (tile32 * 32 + (lane & 31)) * 128 + ((chunk ^ (lane & 7)) * 16));
+            return *(const __attribute__((address_space(3))) s16x8*)(src + (tile32 * 32 + (lane & 31)) * 128 + ((chunk ^ ((lane >> 1) & 7)) * 16));
         }
         constexpr int ROW = N * PL * 2;
         const int granule = tile32 * 2 * PL + plane * 2 + ((lane >> 4) & 1);
         const int row = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
         const lds_char* p = src + row * ROW + ((granule ^ (2 * ((lane >> 2) & 3))) * 32) + (lane & 3) * 8;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * ROW));
+        const s16x4 lo = read_tr(p), hi = read_tr(p + 4 * ROW);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 
-    // One stage multiplied from `now` while stage `blk` (if `more`) is loaded into `next`.  The two buffers are told apart by
-    // __restrict__: without it the compiler waits for the loads into `next` before the first read of `now`.
-    static __device__ __forceinline__ void step(const Tile& tl, const Tile& tr, int blk, bool more, const lds_char* __restrict__ now,
-                                                lds_char* __restrict__ next, int wl, int wr, f32x16 (&acc)[TL][TR]) {
-        if (more) {
-            load<LN, L_RS>(tl, blk, next);
-            load<RN, R_RS>(tr, blk, next + L_BYTES);
-        }
+    struct Frags {
+        s16x8 l[PL][TL], r[PL][TR];
+    };
+
+    static __device__ __forceinline__ void load_stage(const Tile& tl, const Tile& tr, int blk, lds_char* dst) {
+        load<LN, L_RS>(tl, blk, dst);
+        load<RN, R_RS>(tr, blk, dst + L_BYTES);
+    }
+
+    static __device__ __forceinline__ void fetch(const lds_char* src, int kk, int wl, int wr, Frags& f) {
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) {
-            s16x8 fl[PL][TL], fr[PL][TR];
+        for (int p = 0; p < PL; ++p) {
 #pragma unroll
-            for (int p = 0; p < PL; ++p) {
+            for (int b = 0; b < TR; ++b) f.r[p][b] = frag<R_RS, RN>(src + L_BYTES, wr * TR + b, p, kk);
 #pragma unroll
-                for (int a = 0; a < TL; ++a) fl[p][a] = frag<L_RS, LN>(now, wl * TL + a, p, kk);
-#pragma unroll
-                for (int b = 0; b < TR; ++b) fr[p][b] = frag<R_RS, RN>(now + L_BYTES, wr * TR + b, p, kk);
-            }
-#pragma unroll
-            for (int a = 0; a < TL; ++a)
-#pragma unroll
-                for (int b = 0; b < TR; ++b) {
-                    if (PL == 2) {
-                        acc[a][b] = Mma<H>::run(fr[PL - 1][b], fl[0][a], acc[a][b]);
-                        acc[a][b] = Mma<H>::run(fr[0][b], fl[PL - 1][a], acc[a][b]);
-                    }
-                    acc[a][b] = Mma<H>::run(fr[0][b], fl[0][a], acc[a][b]);
-                }
+            for (int a = 0; a < TL; ++a) f.l[p][a] = frag<L_RS, LN>(src, wl * TL + a, p, kk);
         }
     }
 
-    static __device__ __forceinline__ void run(const Tile& tl, const Tile& tr, int blocks, lds_char* smem, f32x16 (&acc)[TL][TR]) {
+    static __device__ __forceinline__ void multiply(const Frags& f, f32x16 (&acc)[TL][TR]) {
+#pragma unroll
+        for (int a = 0; a < TL; ++a)
+#pragma unroll
+            for (int b = 0; b < TR; ++b) {
+                if (PL == 2) {
+                    acc[a][b] = Mma<H>::run(f.r[PL - 1][b], f.l[0][a], acc[a][b]);
+                    acc[a][b] = Mma<H>::run(f.r[0][b], f.l[PL - 1][a], acc[a][b]);
+                }
+                acc[a][b] = Mma<H>::run(f.r[0][b], f.l[0][a], acc[a][b]);
+            }
+    }
+
+    // This wave's loads into LDS have landed and its reads have returned; then everybody's.
+    static __device__ __forceinline__ void meet() {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+
+    // What a workgroup multiplies now, and what next (`more`): the next tile's first stage is loaded during the last one of this.
+    struct Job {
+        Tile l, r;
+        int blocks;
+    };
+    static __device__ __forceinline__ void load_ahead(const Job& job, const Job& next, bool more, int blk, lds_char* dst) {
+        if (blk < job.blocks) load_stage(job.l, job.r, blk, dst);
+        else if (more && blk == job.blocks) load_stage(next.l, next.r, 0, dst);
+    }
+
+    // Stage `blk` from `cur`, its first fragments in f[0] already and stage blk + 1 on its way into `oth`.  The meeting between the
+    // stages lies before the last multiplications of a stage: they cover it, the next stage's first reads and the loads' issue.
+    static __device__ __forceinline__ void stage(const Job& job, const Job& next, bool more, int blk, lds_char* cur, lds_char* oth, int wl,
+                                                 int wr, Frags (&f)[2], f32x16 (&acc)[TL][TR]) {
+#pragma unroll
+        for (int kk = 0; kk + 1 < KS; ++kk) {
+            fetch(cur, kk + 1, wl, wr, f[(kk + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f[kk & 1], acc);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (blk + 1 < job.blocks) {
+            meet();
+            load_ahead(job, next, more, blk + 2, cur);
+            fetch(oth, 0, wl, wr, f[0]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        multiply(f[(KS - 1) & 1], acc);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // Fragments a step ahead (8192 x 8192 x 2048: 1128 TFLOP/s where both operands are RC, against 1066 without; the others
+    // within 2 %).  Two limbs' fragments do not fit the registers twice, so they are read step by step (1230 against 1148).
+    static constexpr bool AHEAD = PL == 1;
+
+    // `buffer`: where the job's first stage is (or goes, unless `primed`); both are carried from job to job.  blocks >= 1.
+    static __device__ __forceinline__ void run(const Job& job, const Job& next, bool more, bool& primed, int& buffer, lds_char* smem,
+                                               f32x16 (&acc)[TL][TR]) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wl = wave / WR, wr = wave % WR;
 #pragma unroll
         for (int a = 0; a < TL; ++a)
 #pragma unroll
             for (int b = 0; b < TR; ++b) acc[a][b] = f32x16{};
-        if (blocks <= 0) return;
-        load<LN, L_RS>(tl, 0, smem);
-        load<RN, R_RS>(tr, 0, smem + L_BYTES);
-        for (int blk = 0; blk < blocks; ++blk) {
-            // this wave's loads of the stage are in LDS; then everybody's are, and everybody is done with the other buffer
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            step(tl, tr, blk + 1, blk + 1 < blocks, smem + (blk & 1) * STAGE, smem + ((blk + 1) & 1) * STAGE, wl, wr, acc);
+        lds_char* even = smem + buffer * STAGE;
+        lds_char* odd = smem + (buffer ^ 1) * STAGE;
+        if (!primed) load_stage(job.l, job.r, 0, even);
+        if (AHEAD) {
+            static_assert(KS % 2 == 0, "a stage's first fragments are those of f[0]");
+            Frags f[2];
+            meet();
+            load_ahead(job, next, more, 1, odd);
+            fetch(even, 0, wl, wr, f[0]);
+            for (int blk = 0; blk < job.blocks; blk += 2) {
+                stage(job, next, more, blk, even, odd, wl, wr, f, acc);
+                if (blk + 1 < job.blocks) stage(job, next, more, blk + 1, odd, even, wl, wr, f, acc);
+            }
+        } else {
+            for (int blk = 0; blk < job.blocks; ++blk) {
+                meet();
+                load_ahead(job, next, more, blk + 1, blk & 1 ? even : odd);
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) {
+                    Frags f;
+                    fetch(blk & 1 ? odd : even, kk, wl, wr, f);
+                    multiply(f, acc);
+                }
+            }
         }
+        primed = more;
+        buffer ^= job.blocks & 1;
     }
 };
+
+// Work items of a launch, dealt to its workgroups: those go round the 8 XCDs one after another, so each XCD gets a contiguous run
+// of items and its workgroups take turns in it.
+struct Deal {
+    long long first, end;
+    int stride;
+    __device__ __forceinline__ Deal(long long count) {
+        const long long x = blockIdx.x & 7, base = count >> 3, extra = count & 7;
+        const long long start = x * base + (x < extra ? x : extra);
+        first = start + (blockIdx.x >> 3);
+        end = start + base + (x < extra ? 1 : 0);
+        stride = (int)((gridDim.x + 7 - x) >> 3);
+    }
+};
+
+// Tile `t` of nrow x ncol: down 8 rows of tiles before the next column, so that the operands of neighbours meet in the L2.
+__device__ __forceinline__ void tile_at(long long t, long long nrow, long long ncol, long long& row, long long& col) {
+    const long long group = t / (8 * ncol), first = group * 8;
+    const long long rows = nrow - first < 8 ? nrow - first : 8;
+    const long long in = t - group * 8 * ncol;
+    row = first + in % rows;
+    col = in / rows;
+}
 
 }  // namespace hgemm

@@ -34,8 +34,8 @@ using hgemm::s16x8;
 using hgemm::Tile;
 
 constexpr int XT = 256;                          // classes a tile
-constexpr long long XE_PIECE_BYTES = 128ll << 20; // dz of a piece: stays in the 256 MB cache between its kernels
-constexpr long long XE_PACK_BYTES = 256ll << 20;  // w of a piece where it has to be packed
+constexpr long long XE_PIECE_BYTES = 512ll << 20; // dz of a piece
+constexpr long long XE_PACK_BYTES = 512ll << 20;  // w of a piece where it has to be packed
 constexpr float XE_DZ_SCALE = 16384.f;           // what dz, below 2 in its units, is multiplied by before it is split
 
 template <int PL>
@@ -61,46 +61,104 @@ __device__ __forceinline__ float xe_scale(unsigned amax_bits) {
     return amax_bits == 0 ? 1.f : __uint_as_float((unsigned)(s > 253 ? 253 : s) << 23);
 }
 
-// ---- scales: the largest finite magnitudes of x (counted rows) and w, as bits
-__global__ void xe_zero_kernel(unsigned* __restrict__ amax) { amax[threadIdx.x] = 0u; }
+// ---- scales: the largest finite magnitudes of x (counted rows) and w.  XE_AMAX workgroups leave one partial maximum each for
+// x (rows dealt round) and for w (chunks); the kernel that packs x, the next one, joins them and leaves the result.
+constexpr int XE_AMAX = 1024;
+
+__device__ __forceinline__ float xe_block_max(float m) {
+    __shared__ float part[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+
+__device__ __forceinline__ float xe_amax_range(const float* __restrict__ p, long long begin, long long end) {
+    const float inf = __builtin_inff();
+    float m = 0.f;
+    auto take = [&](float v) {
+        const float a = fabsf(v);
+        m = a < inf ? fmaxf(m, a) : m;
+    };
+    long long i = begin + threadIdx.x * 4;
+    for (; i + 3 * 1024 + 3 < end; i += 4096) {                 // 64 bytes a thread in flight
+        hgemm::f32x4_any v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const hgemm::f32x4_any*>(p + i + u * 1024);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take(v[u][e]);
+    }
+    for (; i < end; i += 1024)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (i + e < end) take(p[i + e]);
+    return m;
+}
 
 __global__ __launch_bounds__(256) void xe_amax_kernel(const float* __restrict__ X, long long M, long long K,
                                                       const long long* __restrict__ labels, long long ignore,
-                                                      const float* __restrict__ W, long long KV, unsigned* __restrict__ amax) {
-    const bool is_x = blockIdx.y == 0;
-    const float* p = is_x ? X : W;
-    const long long n = is_x ? M * K : KV;
+                                                      const float* __restrict__ W, long long KV, float* __restrict__ partial) {
     float m = 0.f;
-    const long long stride = (long long)gridDim.x * 256;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
-        const float v = fabsf(p[i]);
-        if (v < __builtin_inff() && (!is_x || labels[i / K] != ignore)) m = fmaxf(m, v);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    if ((threadIdx.x & 63) == 0 && m > 0.f) atomicMax(amax + (is_x ? 0 : 1), __float_as_uint(m));   // order does not matter
+    for (long long r = blockIdx.x; r < M; r += XE_AMAX)
+        if (labels[r] != ignore) m = fmaxf(m, xe_amax_range(X, r * K, (r + 1) * K));
+    m = xe_block_max(m);
+    if (threadIdx.x == 0) partial[blockIdx.x] = m;
+    const long long chunk = ((KV + XE_AMAX - 1) / XE_AMAX + 3) / 4 * 4, begin = blockIdx.x * chunk;
+    m = xe_block_max(begin < KV ? xe_amax_range(W, begin, begin + chunk < KV ? begin + chunk : KV) : 0.f);
+    if (threadIdx.x == 0) partial[XE_AMAX + blockIdx.x] = m;
 }
 
-// ---- packing: [rows, cols] of any alignment -> rows of ld halves, zero behind cols; rows labelled `ignore` as zeros
+// ---- packing: [rows, cols] of any alignment -> rows of ld halves, zero behind cols; rows labelled `ignore` as zeros.
+// `partial` (x only): the partial maxima, joined here into amax[0] (x) and amax[1] (w).
 template <typename T, int PL>
 __global__ __launch_bounds__(256) void xe_pack_kernel(const T* __restrict__ src, long long ld_src, long long rows, long long cols,
                                                       short* __restrict__ dst, long long ld, const long long* __restrict__ labels,
-                                                      long long ignore, const unsigned* __restrict__ amax, int vec) {
+                                                      long long ignore, const float* __restrict__ partial, unsigned* __restrict__ amax) {
     const long long per_row = ld / PL / 8;                      // groups of 8 values
     const long long total = rows * per_row;
-    const float scale = PL == 2 ? xe_scale(*amax) : 1.f;
+    float scale = 1.f;
+    if (PL == 2) {
+        if (partial) {
+            float m = 0.f, w = 0.f;
+#pragma unroll
+            for (int k = 0; k < XE_AMAX / 256; ++k) {
+                m = fmaxf(m, partial[k * 256 + threadIdx.x]);
+                w = fmaxf(w, partial[XE_AMAX + k * 256 + threadIdx.x]);
+            }
+            m = xe_block_max(m);
+            if (blockIdx.x == 0) {
+                w = xe_block_max(w);
+                if (threadIdx.x == 0) {
+                    amax[0] = __float_as_uint(m);
+                    amax[1] = __float_as_uint(w);
+                }
+            }
+            scale = xe_scale(__float_as_uint(m));
+        } else {
+            scale = xe_scale(*amax);
+        }
+    }
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const long long r = i / per_row, c = (i - r * per_row) * 8;
         float v[8];
         const bool skip = labels && labels[r] == ignore;
         const T* p = src + r * ld_src + c;
-        if (vec && c + 8 <= cols && !skip) {
+        if (c + 8 <= cols && !skip) {                           // vector loads at the element's alignment
+            if (sizeof(T) == 2) {
+                const s16x8 q = *reinterpret_cast<const hgemm::s16x8_any*>(p);
 #pragma unroll
-            for (int e = 0; e < 8; e += 16 / (int)sizeof(T)) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(p + e);
-                const T* t = reinterpret_cast<const T*>(&q);
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float((unsigned)(unsigned short)q[e] << 16);
+            } else {
+                const f32x4 a = *reinterpret_cast<const hgemm::f32x4_any*>(p), b = *reinterpret_cast<const hgemm::f32x4_any*>(p + 4);
 #pragma unroll
-                for (int j = 0; j < 16 / (int)sizeof(T); ++j) v[e + j] = xe_load(t + j);
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = a[e];
+                    v[4 + e] = b[e];
+                }
             }
         } else {
 #pragma unroll
@@ -125,18 +183,6 @@ __global__ __launch_bounds__(256) void xe_pack_kernel(const T* __restrict__ src,
     }
 }
 
-// Workgroup -> tile.  Workgroups go round the 8 XCDs one after another: each XCD gets a contiguous run of tiles, and within it
-// tiles run down 8 rows of tiles before they move to the next column, so that the operands of neighbours meet in its L2.
-__device__ __forceinline__ void xe_tile_of(long long bid, long long count, long long nrow, long long ncol, long long& row, long long& col) {
-    const long long x = bid & 7, base = count >> 3, extra = count & 7;
-    const long long t = x * base + (x < extra ? x : extra) + (bid >> 3);
-    const long long group = t / (8 * ncol), first = group * 8;
-    const long long rows = nrow - first < 8 ? nrow - first : 8;
-    const long long in = t - group * 8 * ncol;
-    row = first + in % rows;
-    col = in / rows;
-}
-
 // ---- logits of an LN x 256 tile and what the softmax needs of them
 template <int PL, int LN, int WL, int WR>
 __global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
@@ -146,21 +192,31 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
     float* __restrict__ zlab, float* __restrict__ beaten, void* __restrict__ E, long long lde, long long e0, long long e_tiles) {
     typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const long long nrow = (M + LN - 1) / LN, ncol = (vend - v0 + XT - 1) / XT;
-    long long rt, ct;
-    xe_tile_of(blockIdx.x, nrow * ncol, nrow, ncol, rt, ct);
-    const long long m0 = rt * LN, n0 = ct * XT;                 // n0 within the piece
-    const Tile tl = {reinterpret_cast<const char*>(X + m0 * ldx), (M - m0) * ldx * 2, ldx * 2};
-    const Tile tr = {reinterpret_cast<const char*>(W + n0 * PL), w_left - n0 * PL * 2, ldw * 2};
-    f32x16 acc[G::TL][G::TR];
-    G::run(tl, tr, (int)(ldx / 64), (lds_char*)smem, acc);
-    __syncthreads();
-
-    float* sbias = reinterpret_cast<float*>(smem);              // [256]
+    float* sbias = reinterpret_cast<float*>(smem + G::LDS_BYTES);   // [256]
     float* smax = sbias + XT;                                   // [WR][LN]
     float* ssum = smax + WR * LN;                               // [WR][LN]
     float* slab = ssum + WR * LN;                               // [LN]: the labels' logits
     unsigned* sbeat = reinterpret_cast<unsigned*>(slab + LN);   // [LN]
+    const long long nrow = (M + LN - 1) / LN, ncol = (vend - v0 + XT - 1) / XT;
+    auto job_at = [&](long long t, long long& m0, long long& n0) {
+        long long rt, ct;
+        hgemm::tile_at(t, nrow, ncol, rt, ct);
+        m0 = rt * LN, n0 = ct * XT;                             // n0 within the piece
+        return typename G::Job{{reinterpret_cast<const char*>(X + m0 * ldx), (M - m0) * ldx * 2, ldx * 2},
+                               {reinterpret_cast<const char*>(W + n0 * PL), w_left - n0 * PL * 2, ldw * 2},
+                               (int)(ldx / 64)};
+    };
+    const hgemm::Deal deal(nrow * ncol);
+    bool primed = false;
+    int buffer = 0;
+    for (long long t = deal.first; t < deal.end; t += deal.stride) {
+    const bool more = t + deal.stride < deal.end;
+    long long m0, n0, next_m0, next_n0;
+    const typename G::Job job = job_at(t, m0, n0), next = more ? job_at(t + deal.stride, next_m0, next_n0) : job;
+    const long long ct = n0 / XT;
+    f32x16 acc[G::TL][G::TR];
+    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
+
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wl = wave / WR, wr = wave % WR;
     for (int i = tid; i < XT; i += G::THREADS) {
@@ -280,49 +336,57 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
             }
         }
     }
+    __syncthreads();                                            // the tile's statistics have been read
+    }
 }
 
 // ---- the tiles' maxima and sums joined: lse, loss, whether the label has the largest logit (ties to the lowest class).
-// A workgroup takes `rows` rows (a power of two up to 64), 256 / rows threads a row.
+// A workgroup takes `rows` rows (a power of two up to 16: reads of 64 bytes), 256 / rows threads a row.
 __global__ __launch_bounds__(256) void xe_merge_kernel(const float* __restrict__ tmax, const float* __restrict__ tsum, long long ntiles,
                                                        const long long* __restrict__ labels, long long M, long long V, long long ignore,
                                                        int rows, const float* __restrict__ zlab, const float* __restrict__ beaten,
                                                        float* __restrict__ lse, float* __restrict__ loss, float* __restrict__ hit) {
-    __shared__ float red[256];
+    __shared__ float smax[256], ssum[256], slost[256];
     const int lanes = 256 / rows, rl = threadIdx.x % rows, tl = threadIdx.x / rows;
     const long long m = (long long)blockIdx.x * rows + rl;
     const bool live = m < M;
-    float mx = -__builtin_inff();
-    if (live)
-        for (long long t = tl; t < ntiles; t += lanes) mx = fmaxf(mx, tmax[t * M + m]);
-    red[threadIdx.x] = mx;
-    __syncthreads();
-    for (int k = 0; k < lanes; ++k) mx = fmaxf(mx, red[k * rows + rl]);
-    float s = 0.f;
     const long long label = live ? labels[m] : ignore;
-    const bool valid = live && label >= 0 && label < V;
+    const bool valid = live && label != ignore && label >= 0 && label < V;
     const float zl = valid ? zlab[m] : 0.f;
-    float lost = 0.f;
+    const long long own = valid ? label / XT : -1;
+    float mx = -__builtin_inff(), s = 0.f, lost = 0.f;
     if (live)
+#pragma unroll 4
         for (long long t = tl; t < ntiles; t += lanes) {
-            const float v = tmax[t * M + m];
-            s += tsum[t * M + m] * __expf(v - mx);
-            if (t != label / XT && (v > zl || (v == zl && t < label / XT))) lost = 1.f;
+            const float v = tmax[t * M + m], w = tsum[t * M + m];
+            const float top = fmaxf(mx, v), ref = top == -__builtin_inff() ? 0.f : top;
+            s = s * __expf(mx - ref) + w * __expf(v - ref);
+            mx = top;
+            if (t != own && (v > zl || (v == zl && t < own))) lost = 1.f;
         }
+    smax[threadIdx.x] = mx;
+    ssum[threadIdx.x] = s;
+    slost[threadIdx.x] = lost;
     __syncthreads();
-    red[threadIdx.x] = s;
-    __syncthreads();
-    s = 0.f;
-    for (int k = 0; k < lanes; ++k) s += red[k * rows + rl];
-    __syncthreads();
-    red[threadIdx.x] = lost;
-    __syncthreads();
+    for (int half = lanes / 2; half > 0; half /= 2) {           // a tree: the order of the sums is that of the sizes alone
+        if (tl < half) {
+            const int o = threadIdx.x + half * rows;
+            const float v = smax[o], top = fmaxf(mx, v), ref = top == -__builtin_inff() ? 0.f : top;
+            s = s * __expf(mx - ref) + ssum[o] * __expf(v - ref);
+            mx = top;
+            lost += slost[o];
+            smax[threadIdx.x] = mx;
+            ssum[threadIdx.x] = s;
+            slost[threadIdx.x] = lost;
+        }
+        __syncthreads();
+    }
     if (tl != 0 || !live) return;
-    for (int k = 1; k < lanes; ++k) lost += red[k * rows + rl];
-    const float l = mx + logf(s);
+    // a row without any class (all masked) has no loss: NaN, as a sum of zeros gives
+    const float l = mx == -__builtin_inff() ? __builtin_nanf("") : mx + logf(s);
     lse[m] = l;
     loss[m] = label == ignore ? 0.f : valid ? l - zl : __builtin_nanf("");
-    hit[m] = label != ignore && valid && lost == 0.f && beaten[m] == 0.f ? 1.f : 0.f;
+    hit[m] = valid && lost == 0.f && beaten[m] == 0.f ? 1.f : 0.f;
 }
 
 // totals: sum of the losses, counted rows, mean over the counted rows (0 where there are none), hits.  One workgroup, fixed order.
@@ -471,10 +535,18 @@ __device__ __forceinline__ void xe_put(__hip_bfloat16* p, float v) { *p = __floa
 template <typename T>
 __global__ __launch_bounds__(256) void xe_db_kernel(const float* __restrict__ dbp, long long blocks, long long ld, long long cols,
                                                     const float* __restrict__ scale, T* __restrict__ DB) {
-    const long long n = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (n >= cols) return;
+    __shared__ double part[8][32];
+    const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const long long n = (long long)blockIdx.x * 32 + cl;
     double s = 0.0;
-    for (long long r = 0; r < blocks; ++r) s += (double)dbp[r * ld + n];
+    if (n < cols)
+#pragma unroll 4
+        for (long long r = rl; r < blocks; r += 8) s += (double)dbp[r * ld + n];
+    part[rl][cl] = s;
+    __syncthreads();
+    if (rl != 0 || n >= cols) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += part[k][cl];
     xe_put(DB + n, (float)s * *scale);
 }
 
@@ -486,15 +558,27 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_dx_kernel(const short* __rest
     typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long nrow = (M + LN - 1) / LN, ncol = (K + XT - 1) / XT, tiles = nrow * ncol;
-    const int split = (int)(blockIdx.x / tiles);
-    long long rt, ct;
-    xe_tile_of(blockIdx.x - split * tiles, tiles, nrow, ncol, rt, ct);
-    const int b0 = (int)((long long)blocks * split / splits), b1 = (int)((long long)blocks * (split + 1) / splits);
-    const long long m0 = rt * LN, k0 = ct * XT, skip = (long long)b0 * 128;
-    const Tile tl = {reinterpret_cast<const char*>(dz + m0 * ldz) + skip, (M - m0) * ldz * 2 - skip, ldz * 2};
-    const Tile tr = {reinterpret_cast<const char*>(W + k0 * ldw) + skip, w_left - k0 * ldw * 2 - skip, ldw * 2};
+    auto job_at = [&](long long t, long long& m0, long long& k0, int& split) {
+        long long rt, ct;
+        split = (int)(t / tiles);
+        hgemm::tile_at(t - split * tiles, nrow, ncol, rt, ct);
+        m0 = rt * LN, k0 = ct * XT;
+        const int b0 = (int)((long long)blocks * split / splits), b1 = (int)((long long)blocks * (split + 1) / splits);
+        const long long skip = (long long)b0 * 128;
+        return typename G::Job{{reinterpret_cast<const char*>(dz + m0 * ldz) + skip, (M - m0) * ldz * 2 - skip, ldz * 2},
+                               {reinterpret_cast<const char*>(W + k0 * ldw) + skip, w_left - k0 * ldw * 2 - skip, ldw * 2},
+                               b1 - b0};
+    };
+    const hgemm::Deal deal(tiles * splits);
+    bool primed = false;
+    int buffer = 0;
+    for (long long t = deal.first; t < deal.end; t += deal.stride) {
+    const bool more = t + deal.stride < deal.end;
+    long long m0, k0, next_m0, next_k0;
+    int split, next_split;
+    const typename G::Job job = job_at(t, m0, k0, split), next = more ? job_at(t + deal.stride, next_m0, next_k0, next_split) : job;
     f32x16 acc[G::TL][G::TR];
-    G::run(tl, tr, b1 - b0, (lds_char*)smem, acc);
+    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
 #pragma unroll
     for (int a = 0; a < G::TL; ++a) {
@@ -511,6 +595,7 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_dx_kernel(const short* __rest
                 if (accumulate) v += *reinterpret_cast<const f32x4*>(out);
                 *reinterpret_cast<f32x4*>(out) = v;
             }
+    }
     }
 }
 
@@ -536,13 +621,23 @@ __global__ __launch_bounds__(512) void xe_dw_kernel(const short* __restrict__ X,
     typedef Gemm<typename HalfOf<PL>::type, PL, 256, XT, 2, 4, true, true> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long nrow = (K + 255) / 256, ncol = (cols + XT - 1) / XT;
-    long long rt, ct;
-    xe_tile_of(blockIdx.x, nrow * ncol, nrow, ncol, rt, ct);
-    const long long k0 = rt * 256, n0 = ct * XT;
-    const Tile tl = {reinterpret_cast<const char*>(X + k0 * PL), M * ldx * 2 - k0 * PL * 2, ldx * 2};
-    const Tile tr = {reinterpret_cast<const char*>(dz + n0 * PL), M * ldz * 2 - n0 * PL * 2, ldz * 2};
+    auto job_at = [&](long long t, long long& k0, long long& n0) {
+        long long rt, ct;
+        hgemm::tile_at(t, nrow, ncol, rt, ct);
+        k0 = rt * 256, n0 = ct * XT;
+        return typename G::Job{{reinterpret_cast<const char*>(X + k0 * PL), M * ldx * 2 - k0 * PL * 2, ldx * 2},
+                               {reinterpret_cast<const char*>(dz + n0 * PL), M * ldz * 2 - n0 * PL * 2, ldz * 2},
+                               (int)((M + G::CB - 1) / G::CB)};
+    };
+    const hgemm::Deal deal(nrow * ncol);
+    bool primed = false;
+    int buffer = 0;
+    for (long long t = deal.first; t < deal.end; t += deal.stride) {
+    const bool more = t + deal.stride < deal.end;
+    long long k0, n0, next_k0, next_n0;
+    const typename G::Job job = job_at(t, k0, n0), next = more ? job_at(t + deal.stride, next_k0, next_n0) : job;
     f32x16 acc[G::TL][G::TR];
-    G::run(tl, tr, (int)((M + G::CB - 1) / G::CB), (lds_char*)smem, acc);
+    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
     const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) / XE_DZ_SCALE : 1.f;
     const float g = *scale;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / 4, wr = wave % 4;
@@ -584,6 +679,7 @@ __global__ __launch_bounds__(512) void xe_dw_kernel(const short* __restrict__ X,
                     }
                 }
         }
+    }
     }
 }
 
@@ -642,7 +738,7 @@ struct Carver {
 
 struct FwdBuffers {
     short *x, *w;
-    float *tsum, *beaten, *hit;
+    float *tsum, *beaten, *hit, *partial;
     long long bytes;
     FwdBuffers(const Plan& p, void* ws) {
         Carver c(ws);
@@ -651,6 +747,7 @@ struct FwdBuffers {
         tsum = c.take<float>(p.M * p.tiles);
         beaten = c.take<float>(p.M);
         hit = c.take<float>(p.M);
+        partial = c.take<float>(2 * XE_AMAX);
         bytes = c.used;
     }
 };
@@ -674,6 +771,9 @@ struct BwdBuffers {
     long long bytes;
 };
 
+// One workgroup a compute unit where the tiles take most of its LDS, two where they take half.
+unsigned grid_for(long long items, int lds) { return (unsigned)lowest(items, lds > (80 << 10) ? 256 : 512); }
+
 template <typename F>
 int with_lds(F* kernel, int bytes) {
     return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -686,25 +786,24 @@ int with_lds(F* kernel, int bytes) {
     } while (0)
 
 int pack(const Plan& p, const void* src, long long ld_src, long long rows, long long cols, short* dst, long long ld,
-         const long long* labels, long long ignore, const unsigned* amax, hipStream_t stream) {
+         const long long* labels, long long ignore, const float* partial, unsigned* amax, hipStream_t stream) {
     const long long total = rows * (ld / p.pl / 8);
     const unsigned grid = (unsigned)lowest((total + 255) / 256, 8192);
-    const int align = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld_src % (p.type ? 8 : 4) == 0;
     if (p.type == 1)
         hipLaunchKernelGGL((xe_pack_kernel<__hip_bfloat16, 1>), dim3(grid), dim3(256), 0, stream,
-                           static_cast<const __hip_bfloat16*>(src), ld_src, rows, cols, dst, ld, labels, ignore, amax, align);
+                           static_cast<const __hip_bfloat16*>(src), ld_src, rows, cols, dst, ld, labels, ignore, partial, amax);
     else if (p.pl == 1)
         hipLaunchKernelGGL((xe_pack_kernel<float, 1>), dim3(grid), dim3(256), 0, stream, static_cast<const float*>(src), ld_src, rows,
-                           cols, dst, ld, labels, ignore, amax, align);
+                           cols, dst, ld, labels, ignore, partial, amax);
     else
         hipLaunchKernelGGL((xe_pack_kernel<float, 2>), dim3(grid), dim3(256), 0, stream, static_cast<const float*>(src), ld_src, rows,
-                           cols, dst, ld, labels, ignore, amax, align);
+                           cols, dst, ld, labels, ignore, partial, amax);
     DTF_CHECK_LAUNCH();
     return 0;
 }
 
 // w of the classes [v0, v0 + cols): packed into `buf`, or in place.  *left: bytes from there to the end of the operand.
-int piece_of_w(const Plan& p, const void* W, long long v0, long long cols, short* buf, const unsigned* amax, hipStream_t stream,
+int piece_of_w(const Plan& p, const void* W, long long v0, long long cols, short* buf, unsigned* amax, hipStream_t stream,
                const short** w, long long* left) {
     const char* src = static_cast<const char*>(W) + v0 * (p.type ? 2 : 4);
     if (!p.packs) {
@@ -714,7 +813,7 @@ int piece_of_w(const Plan& p, const void* W, long long v0, long long cols, short
     }
     *w = buf;
     *left = p.K * p.ldw * 2;
-    return pack(p, src, p.V, p.K, cols, buf, p.ldw, nullptr, 0, amax + 1, stream);
+    return pack(p, src, p.V, p.K, cols, buf, p.ldw, nullptr, 0, nullptr, amax + 1, stream);
 }
 
 struct Call {
@@ -730,9 +829,10 @@ int launch_logits(const Plan& p, const Call& c, const short* x, const short* w, 
                   long long e_tiles) {
     typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
     auto* kernel = &xe_logits_kernel<PL, LN, WL, WR>;
-    XE_TRY(with_lds(kernel, G::LDS_BYTES));
+    constexpr int lds = G::LDS_BYTES + (XT + 2 * WR * LN + 2 * LN) * 4;
+    XE_TRY(with_lds(kernel, lds));
     const long long tiles = ((p.M + LN - 1) / LN) * ((vend - v0 + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(G::THREADS), G::LDS_BYTES, c.stream, x, p.ldx, w, p.ldw, left, c.B,
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles, lds)), dim3(G::THREADS), lds, c.stream, x, p.ldx, w, p.ldw, left, c.B,
                        p.type, c.labels, p.M, p.K, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
     DTF_CHECK_LAUNCH();
     return 0;
@@ -754,8 +854,9 @@ int launch_dx(const Plan& p, const short* dz, const short* w, long long left, lo
     auto* kernel = &xe_dx_kernel<PL, LN, WL, WR>;
     XE_TRY(with_lds(kernel, G::LDS_BYTES));
     const long long tiles = ((p.M + LN - 1) / LN) * ((p.K + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * p.splits)), dim3(G::THREADS), G::LDS_BYTES, stream, dz, p.piece * PL, w, p.ldw,
-                       left, p.M, p.K, (int)((cols + G::CB - 1) / G::CB), p.splits, !first, slab, p.ldk);
+    const int blocks = (int)((cols + G::CB - 1) / G::CB), splits = (int)lowest(p.splits, blocks);   // (a last piece may be short)
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles * splits, G::LDS_BYTES)), dim3(G::THREADS), G::LDS_BYTES, stream, dz, p.piece * PL, w,
+                       p.ldw, left, p.M, p.K, blocks, splits, !first, slab, p.ldk);
     DTF_CHECK_LAUNCH();
     return 0;
 }
@@ -767,7 +868,7 @@ int launch_dw(const Plan& p, const short* x, const short* dz, long long v0, long
     auto* kernel = &xe_dw_kernel<PL, OUT_BF16>;
     XE_TRY(with_lds(kernel, G::LDS_BYTES));
     const long long tiles = ((p.K + 255) / 256) * ((cols + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles, G::LDS_BYTES)), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
                        cols, amax, scale, DW, p.V, v0);
     DTF_CHECK_LAUNCH();
     return 0;
@@ -777,16 +878,12 @@ int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, 
             long long kept_cols, void* ws) {
     const FwdBuffers b(p, ws);
     if (p.pl == 2) {
-        hipLaunchKernelGGL(xe_zero_kernel, dim3(1), dim3(2), 0, c.stream, amax);
-        DTF_CHECK_LAUNCH();
-        hipLaunchKernelGGL(xe_amax_kernel, dim3(1024, 2), dim3(256), 0, c.stream, static_cast<const float*>(c.X), p.M, p.K, c.labels,
-                           c.ignore, static_cast<const float*>(c.W), p.K * p.V, amax);
+        hipLaunchKernelGGL(xe_amax_kernel, dim3(XE_AMAX), dim3(256), 0, c.stream, static_cast<const float*>(c.X), p.M, p.K, c.labels,
+                           c.ignore, static_cast<const float*>(c.W), p.K * p.V, b.partial);
         DTF_CHECK_LAUNCH();
     }
-    XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, amax, c.stream));
-    // where w is read in place the whole vocabulary is one launch (bounded by the grid: 4194304 tiles)
-    const long long rowtiles = (p.M + (p.small ? 63 : 255)) / (p.small ? 64 : 256);
-    const long long step = p.packs ? p.piece : lowest(p.V, (1 << 22) / rowtiles * XT);
+    XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, b.partial, amax, c.stream));
+    const long long step = p.packs ? p.piece : p.V;             // where w is read in place the whole vocabulary is one launch
     for (long long v0 = 0; v0 < p.V; v0 += step) {
         const long long cols = lowest(step, p.V - v0);
         const short* w;
@@ -795,7 +892,7 @@ int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, 
         const long long e_tiles = kept_cols > v0 ? (kept_cols - v0) / XT : 0;
         XE_TRY(logits(p, c, b.x, w, left, v0, v0 + cols, amax, tmax, b.tsum, zlab, b.beaten, kept, kept_cols, v0, e_tiles));
     }
-    int rows = 64;
+    int rows = 16;
     while (rows > 1 && rows / 2 >= p.M) rows /= 2;
     hipLaunchKernelGGL(xe_merge_kernel, dim3((unsigned)((p.M + rows - 1) / rows)), dim3(256), 0, c.stream, tmax, b.tsum, p.tiles,
                        c.labels, p.M, p.V, c.ignore, rows, zlab, b.beaten, lse, loss, b.hit);
@@ -805,13 +902,13 @@ int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, 
     return 0;
 }
 
-int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, float* tmax, const float* totals, const unsigned* amax,
+int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, float* tmax, const float* totals, unsigned* amax,
              const void* kept, long long kept_cols, int mean, const float* dloss, int stride, void* DX, void* DW, void* DB, void* ws) {
     const BwdBuffers b(p, ws);
     hipLaunchKernelGGL(xe_weights_kernel, dim3(1), dim3(1024), 0, c.stream, dloss, stride, totals, mean, c.labels, p.M, p.V, c.ignore,
                        lse, zlab, b.rowg, b.scale);
     DTF_CHECK_LAUNCH();
-    if (DW || kept_cols < p.V) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, amax, c.stream));
+    if (DW || kept_cols < p.V) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, nullptr, amax, c.stream));
     const long long rowblocks = (p.M + 63) / 64;
     for (long long v0 = 0; v0 < p.V; v0 += p.piece) {
         const long long cols = lowest(p.piece, p.V - v0), ct = (cols + XT - 1) / XT;
@@ -856,7 +953,7 @@ int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, 
             else XE_TRY((launch_dw<1, 0>(p, b.x, b.dz, v0, cols, amax, b.scale, DW, c.stream)));
         }
         if (DB) {
-            const dim3 grid((unsigned)((cols + 255) / 256));
+            const dim3 grid((unsigned)((cols + 31) / 32));
             if (p.type == 1)
                 hipLaunchKernelGGL(xe_db_kernel<__hip_bfloat16>, grid, dim3(256), 0, c.stream, b.dbp, rowblocks, p.piece, cols, b.scale,
                                    static_cast<__hip_bfloat16*>(DB) + v0);
@@ -915,7 +1012,7 @@ DTF_API int dtf_linear_xent_fwd(const void* X, const void* W, const void* B, con
 // rows.  DX, DW, DB may each be null.
 DTF_API int dtf_linear_xent_bwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
                                 long long V, int type, int bf16, long long ignore, const float* lse, const float* zlab, float* tmax,
-                                const float* totals, const unsigned* amax, const void* kept, long long kept_cols, int mean,
+                                const float* totals, unsigned* amax, const void* kept, long long kept_cols, int mean,
                                 const float* dloss, int dloss_stride, void* DX, void* DW, void* DB, void* workspace,
                                 hipStream_t stream) {
     if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
