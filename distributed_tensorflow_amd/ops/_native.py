@@ -88,7 +88,7 @@ def kernels():
         "dtf_softmax_rows": [c_p, c_p, c_i, c_i, c_p],
         "dtf_global_norm_partials": [],
         "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, c_f, c_p, c_p, c_p],
-        "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p],
+        "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p, c_p],
         "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
         "dtf_linear_xent_supported": [c_ll] * 3,
         "dtf_linear_xent_fwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 7 + [c_ll, c_p, c_p],
@@ -125,7 +125,7 @@ def kernels():
             fn = getattr(lib, name)
             fn.argtypes = argtypes
             fn.restype = c_i
-    for name, argtypes in {"dtf_groupnorm_workspace_floats": [c_ll, c_ll, c_i, c_i],
+    for name, argtypes in {"dtf_groupnorm_workspace_doubles": [c_ll, c_ll, c_i, c_i],
                            "dtf_linear_xent_fwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i],
                            "dtf_linear_xent_bwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i]}.items():
         declare(lib, name, argtypes, c_ll)

@@ -352,6 +352,8 @@ def _groupnorm_sizes(x, groups, gamma, beta, *others):
     C = int(x.shape[-1])
     if groups < 1 or C < 1 or C % groups:
         raise ValueError("%d channels do not divide into %d groups" % (C, groups))
+    if C > (1 << 20) or x.shape[0] > (1 << 21):
+        raise ValueError("group normalisation takes at most 2097152 samples and 1048576 channels, got %s" % (tuple(x.shape),))
     for name, t in (("gamma", gamma), ("beta", beta)):
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()
                               or t.device != x.device):
@@ -384,8 +386,10 @@ def groupnorm_forward(x, gamma, beta, groups, eps=1e-3, act=ACT_NONE, out=None, 
         return out, stats
     if x.is_cuda:
         with nv.device_guard(x):
-            rc = nv.kernels().dtf_groupnorm_fwd(nv.ptr(x), nv.ptr(out), B, S, C, groups, _GROUPNORM_TYPES[x.dtype], nv.ptr(gamma),
-                                                nv.ptr(beta), float(eps), int(act), nv.ptr(stats), nv.stream_ptr())
+            lib, kind = nv.kernels(), _GROUPNORM_TYPES[x.dtype]
+            ws = torch.empty(int(lib.dtf_groupnorm_workspace_doubles(B, S, C, kind)), dtype=torch.float64, device=x.device)
+            rc = lib.dtf_groupnorm_fwd(nv.ptr(x), nv.ptr(out), B, S, C, groups, kind, nv.ptr(gamma), nv.ptr(beta), float(eps),
+                                       int(act), nv.ptr(stats), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_groupnorm_fwd")
         return out, stats
     v = x.to(torch.float64).view(B, S, groups, C // groups)
@@ -423,10 +427,9 @@ def groupnorm_backward(x, dy, gamma, beta, groups, stats, act=ACT_NONE, dgamma=N
         return dx
     if x.is_cuda:
         with nv.device_guard(x):
-            lib = nv.kernels()
-            ws = torch.empty(int(lib.dtf_groupnorm_workspace_floats(B, S, C, groups)), dtype=torch.float32, device=x.device)
-            rc = lib.dtf_groupnorm_bwd(nv.ptr(x), nv.ptr(dy), nv.ptr(dx), B, S, C, groups, _GROUPNORM_TYPES[x.dtype],
-                                       nv.ptr(gamma), nv.ptr(beta), int(act), nv.ptr(stats), nv.ptr(dgamma), nv.ptr(dbeta),
+            lib, kind = nv.kernels(), _GROUPNORM_TYPES[x.dtype]
+            ws = torch.empty(int(lib.dtf_groupnorm_workspace_doubles(B, S, C, kind)), dtype=torch.float64, device=x.device)
+            rc = lib.dtf_groupnorm_bwd(nv.ptr(x), nv.ptr(dy), nv.ptr(dx), B, S, C, groups, kind, nv.ptr(gamma), nv.ptr(beta), int(act), nv.ptr(stats), nv.ptr(dgamma), nv.ptr(dbeta),
                                        nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_groupnorm_bwd")
         return dx
