@@ -87,7 +87,7 @@ def kernels():
         "dtf_batchnorm_bwd": [c_p, c_p, c_p, c_ll, c_i, c_p, c_p, c_p, c_p, c_p, c_p, c_p],
         "dtf_softmax_rows": [c_p, c_p, c_i, c_i, c_p],
         "dtf_global_norm_partials": [],
-        "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, c_f, c_p, c_p, c_p],
+        "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, C.c_double, c_p, c_p, c_p],
         "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p, c_p],
         "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
         "dtf_linear_xent_supported": [c_ll] * 3,

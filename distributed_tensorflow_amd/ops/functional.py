@@ -14,9 +14,10 @@ and the Adam apply).
 from __future__ import annotations
 
 import collections
-import ctypes
 import math
+import operator
 
+import numpy as np
 import torch
 
 from . import _native as nv
@@ -721,30 +722,30 @@ def categorical_accuracy_sum(p, y, acc_sum):
 
 # --------------------------------------------------------------------------- global norm over a list of gradients
 _NORM_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NORM_SIZES = np.array([4, 2, 2])
+_DTYPE_OF = operator.attrgetter("dtype")
 
 
-def _norm_list(tensors):
-    """The list's tensors without its None entries, checked."""
-    live = [t for t in tensors if t is not None]
-    for t in live:
-        if t.dtype not in _NORM_TYPES or not t.is_contiguous() or t.device != live[0].device:
-            raise ValueError("the global norm takes contiguous float32, bfloat16 and float16 tensors on one device, got %s %s on %s"
-                             % (t.dtype, tuple(t.stride()), t.device))
-    return live
-
-
-def _norm_launch(live, dst, clip):
+def _norm_table(live):
+    """Addresses, element counts and types of a list's tensors as arrays, after their checks.  Lists of hundreds of gradients
+    are ordinary: the attributes are read by ``map`` over the bound C functions, not in a loop of Python."""
     n = len(live)
-    with nv.device_guard(live[0]):
+    types = list(map(_NORM_TYPES.get, map(_DTYPE_OF, live)))
+    if None in types or not all(map(torch.Tensor.is_contiguous, live)) or len(set(map(torch.Tensor.get_device, live))) != 1:
+        raise ValueError("the global norm takes contiguous float32, bfloat16 and float16 tensors on one device, got %s"
+                         % sorted({"%s %s on %s" % (t.dtype, "contiguous" if t.is_contiguous() else "strided", t.device) for t in live}))
+    return (np.fromiter(map(torch.Tensor.data_ptr, live), np.int64, n), np.fromiter(map(torch.Tensor.numel, live), np.int64, n),
+            np.array(types, np.int8))
+
+
+def _norm_launch(device, src, dst, clip):
+    address = lambda a: a.__array_interface__["data"][0]
+    with nv.device_guard(device):
         lib = nv.kernels()
-        partials = torch.empty(int(lib.dtf_global_norm_partials()), dtype=torch.float64, device=live[0].device)
-        norm = torch.empty((), dtype=torch.float32, device=live[0].device)
-        table = lambda kind, values: (kind * n)(*values)
-        rc = lib.dtf_global_norm(table(ctypes.c_longlong, [t.data_ptr() for t in live]),
-                                 None if dst is None else table(ctypes.c_longlong, [t.data_ptr() for t in dst]),
-                                 table(ctypes.c_longlong, [t.numel() for t in live]),
-                                 table(ctypes.c_byte, [_NORM_TYPES[t.dtype] for t in live]), n, float(clip), nv.ptr(partials),
-                                 nv.ptr(norm), nv.stream_ptr())
+        partials = torch.empty(int(lib.dtf_global_norm_partials()), dtype=torch.float64, device=device.device)
+        norm = torch.empty((), dtype=torch.float32, device=device.device)
+        rc = lib.dtf_global_norm(address(src[0]), None if dst is None else address(dst[0]), address(src[1]), address(src[2]),
+                                 len(src[0]), float(clip), nv.ptr(partials), nv.ptr(norm), nv.stream_ptr())
     nv.check(rc, "dtf_global_norm")
     return norm
 
@@ -752,11 +753,12 @@ def _norm_launch(live, dst, clip):
 def global_norm(tensors):
     """``tf.global_norm``: the square root of the sum of all squares over a list of tensors (float32, bfloat16, float16; None
     entries count for nothing), as a float32 scalar tensor.  Summed in 64 bits and in a fixed order."""
-    live = _norm_list(tensors)
+    live = [t for t in tensors if t is not None]
     if not live:
         return torch.zeros((), dtype=torch.float32)
+    table = _norm_table(live)
     if live[0].is_cuda:
-        return _norm_launch(live, None, math.inf)
+        return _norm_launch(live[0], table, None, math.inf)
     return torch.stack([t.double().square().sum() for t in live]).sum().sqrt().float()
 
 
@@ -764,35 +766,47 @@ def clip_by_global_norm(tensors, clip_norm, out=None):
     """``tf.clip_by_global_norm``: ``([t * clip_norm / max(norm, clip_norm) for t in tensors], norm)`` with the global norm of
     the unclipped list.  None entries stay None.  If the norm is not finite, every output is NaN.
 
-    ``out``: tensors to write into, like ``tensors`` (the list itself: in place, and nothing is written when nothing has to
-    be clipped); no two of them may share memory."""
+    ``out``: tensors to write into, one of the same type and element count for each of ``tensors`` (the list itself: in
+    place, and nothing is written when nothing has to be clipped).  No two of them may share memory, nor one with another
+    entry's input."""
     clip_norm = float(clip_norm)
     if not clip_norm > 0.0:
         raise ValueError("clip_norm must be positive, got %r" % clip_norm)
     tensors = list(tensors)
-    live = _norm_list(tensors)
-    if out is None:
-        out = [None if t is None else torch.empty_like(t) for t in tensors]
-    else:
-        out = list(out)
-        if len(out) != len(tensors) or any((o is None) != (t is None) for o, t in zip(out, tensors)):
-            raise ValueError("out must have a tensor for every tensor of the list")
+    live = [t for t in tensors if t is not None]
+    given = out is not None
+    out = list(out) if given else [None if t is None else torch.empty_like(t) for t in tensors]
     dst = [o for o in out if o is not None]
-    for o, t in zip(dst, live):
-        if o.dtype != t.dtype or o.shape != t.shape or o.device != t.device or not o.is_contiguous():
-            raise ValueError("every tensor of out must be contiguous and like its tensor of the list")
-    spans = sorted((o.data_ptr(), o.data_ptr() + o.numel() * o.element_size()) for o in dst if o.numel())
-    if any(a[1] > b[0] for a, b in zip(spans[:-1], spans[1:])):
-        raise ValueError("two tensors of out share memory")
+    if len(out) != len(tensors) or len(dst) != len(live) or (len(dst) != len(out) and
+                                                             any((o is None) != (t is None) for o, t in zip(out, tensors))):
+        raise ValueError("out must have a tensor for every tensor of the list")
     if not live:
         return out, torch.zeros((), dtype=torch.float32)
+    src = _norm_table(live)
+    table = _norm_table(dst) if given else (np.fromiter(map(torch.Tensor.data_ptr, dst), np.int64, len(dst)),) + src[1:]
+    if given:
+        if not (np.array_equal(table[1], src[1]) and np.array_equal(table[2], src[2])) or live[0].device != dst[0].device:
+            raise ValueError("every tensor of out must be contiguous and like its tensor of the list")
+        size = src[1] * _NORM_SIZES[src[2]]
+        full = size > 0
+        start, end = table[0][full], (table[0] + size)[full]
+        order = np.argsort(start, kind="stable")
+        if (end[order][:-1] > start[order][1:]).any():
+            raise ValueError("two tensors of out share memory")
+        # an output over another entry's input: the inputs that begin or end inside an output that is not theirs
+        begin = src[0][full]
+        other = begin != start
+        if other.any():
+            at = np.searchsorted(start[order], (begin + size[full])[other], side="left") - 1
+            if (end[order][at] > begin[other])[at >= 0].any():
+                raise ValueError("a tensor of out shares memory with an input that is not its own")
     if live[0].is_cuda:
-        return out, _norm_launch(live, dst, clip_norm)
+        return out, _norm_launch(live[0], src, table, clip_norm)
     norm = torch.stack([t.double().square().sum() for t in live]).sum().sqrt()
     v = float(norm)
     f = math.nan if not math.isfinite(v) else 1.0 if v <= clip_norm else clip_norm / v
     for o, t in zip(dst, live):
-        o.copy_((t.float() * f).to(t.dtype) if f != 1.0 else t)
+        o.copy_((t.float() * f).to(t.dtype).view(o.shape) if f != 1.0 else t.view(o.shape))
     return out, norm.float()
 
 
