@@ -88,13 +88,14 @@ struct Tile {
     long long left, ld;
 };
 
-template <typename H, int PL, int LN, int RN, int WL, int WR, bool L_RS, bool R_RS>
+template <typename H, int PL, int LN, int RN, int WL, int WR, bool L_RS, bool R_RS, int STAGES = 2>
 struct Gemm {
     static constexpr int THREADS = 64 * WL * WR, WAVES = WL * WR;
     static constexpr int CB = 64 / PL;                       // values of the reduction a stage
     static constexpr int TL = LN / WL / 32, TR = RN / WR / 32;
     static constexpr int L_BYTES = LN * 128, R_BYTES = RN * 128, STAGE = L_BYTES + R_BYTES;
-    static constexpr int LDS_BYTES = 2 * STAGE;
+    static constexpr int LDS_BYTES = STAGES * STAGE;
+    static constexpr int LOADS = (LN + RN) / 8 / WAVES;      // a wave and stage, 1 KB each
     static constexpr int KS = CB / 16;                       // MFMA steps a stage and limb product
     static_assert(LN % (32 * WL) == 0 && RN % (32 * WR) == 0 && (LN / 8) % WAVES == 0 && (RN / 8) % WAVES == 0, "tile");
     static_assert((!L_RS || LN == 256) && (!R_RS || RN == 256), "the RS layout's banks are worked out for rows of 256 values");
@@ -222,9 +223,38 @@ struct Gemm {
         __builtin_amdgcn_sched_barrier(0);
     }
 
+    // Tiles of few rows: so little to multiply that a stage takes as long as its loads' way, so STAGES - 1 stages are on their way at
+    // a time (128 rows, 512 features, 10001 classes, fp32: @SMALL@).  The loads of stages behind the last
+    // one are issued all the same, out of bounds, so that the number in flight is a constant.
+    static __device__ __forceinline__ void ring(const Job& job, int wl, int wr, lds_char* smem, f32x16 (&acc)[TL][TR]) {
+        const Tile none_l = {job.l.base, 0, job.l.ld}, none_r = {job.r.base, 0, job.r.ld};
+        auto issue = [&](int blk, int at) {
+            if (blk < job.blocks) load_stage(job.l, job.r, blk, smem + at * STAGE);
+            else load_stage(none_l, none_r, 0, smem + at * STAGE);
+        };
+        meet();                                              // nobody reads a buffer of an earlier job any more
+#pragma unroll
+        for (int k = 0; k < STAGES - 1; ++k) issue(k, k);
+        int now = 0, ahead = STAGES - 1;
+        for (int blk = 0; blk < job.blocks; ++blk) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * LOADS) : "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            issue(blk + STAGES - 1, ahead);
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                Frags f;
+                fetch(smem + now * STAGE, kk, wl, wr, f);
+                multiply(f, acc);
+            }
+            now = now + 1 == STAGES ? 0 : now + 1;
+            ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
+        }
+    }
+
     // Fragments a step ahead (8192 x 8192 x 2048: 1128 TFLOP/s where both operands are RC, against 1066 without; the others
     // within 2 %).  Two limbs' fragments do not fit the registers twice, so they are read step by step (1230 against 1148).
-    static constexpr bool AHEAD = PL == 1;
+    static constexpr bool AHEAD = PL == 1 && STAGES == 2;
 
     // `buffer`: where the job's first stage is (or goes, unless `primed`); both are carried from job to job.  blocks >= 1.
     static __device__ __forceinline__ void run(const Job& job, const Job& next, bool more, bool& primed, int& buffer, lds_char* smem,
@@ -235,6 +265,10 @@ struct Gemm {
         for (int a = 0; a < TL; ++a)
 #pragma unroll
             for (int b = 0; b < TR; ++b) acc[a][b] = f32x16{};
+        if (STAGES > 2) {
+            ring(job, wl, wr, smem, acc);
+            return;
+        }
         lds_char* even = smem + buffer * STAGE;
         lds_char* odd = smem + (buffer ^ 1) * STAGE;
         if (!primed) load_stage(job.l, job.r, 0, even);

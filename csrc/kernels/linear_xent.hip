@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
     const void* __restrict__ bias, int bias_bf16, const long long* __restrict__ labels, long long M, long long K, long long v0,
     long long vend, const unsigned* __restrict__ amax, float* __restrict__ tmax, float* __restrict__ tsum,
     float* __restrict__ zlab, float* __restrict__ beaten, void* __restrict__ E, long long lde, long long e0, long long e_tiles) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true, LN == 64 ? 3 : 2> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* sbias = reinterpret_cast<float*>(smem + G::LDS_BYTES);   // [256]
     float* smax = sbias + XT;                                   // [WR][LN]
@@ -389,10 +389,11 @@ __global__ __launch_bounds__(256) void xe_merge_kernel(const float* __restrict__
     hit[m] = valid && lost == 0.f && beaten[m] == 0.f ? 1.f : 0.f;
 }
 
-// totals: sum of the losses, counted rows, mean over the counted rows (0 where there are none), hits.  One workgroup, fixed order.
+// totals: sum of the losses, hits, counted rows, mean over the counted rows (0 where there are none); reduced (may be null): the
+// mean (reduction 1) or the sum (2).  One workgroup, fixed order.
 __global__ __launch_bounds__(1024) void xe_total_kernel(const float* __restrict__ loss, const float* __restrict__ hit,
                                                         const long long* __restrict__ labels, long long M, long long ignore,
-                                                        float* __restrict__ totals) {
+                                                        float* __restrict__ totals, int reduction, float* __restrict__ reduced) {
     __shared__ double part[3][16];
     double s = 0.0, n = 0.0, h = 0.0;
     for (long long m = threadIdx.x; m < M; m += 1024) {
@@ -420,9 +421,10 @@ __global__ __launch_bounds__(1024) void xe_total_kernel(const float* __restrict_
             h += part[2][k];
         }
         totals[0] = (float)s;
-        totals[1] = (float)n;
-        totals[2] = (float)(s / fmax(n, 1.0));
-        totals[3] = (float)h;
+        totals[1] = (float)h;
+        totals[2] = (float)n;
+        totals[3] = (float)(s / fmax(n, 1.0));
+        if (reduced) *reduced = reduction == 1 ? totals[3] : totals[0];
     }
 }
 
@@ -455,21 +457,22 @@ __global__ __launch_bounds__(1024) void xe_weights_kernel(const float* __restric
     const float down = __uint_as_float((unsigned)(127 - unit) << 23);
     for (long long i = threadIdx.x; i < M; i += 1024) rowg[i] *= down;
     if (threadIdx.x == 0)
-        *scale = (stride ? 1.f : *dloss) * (mean ? 1.f / fmaxf(totals[1], 1.f) : 1.f) * __uint_as_float((unsigned)(127 + unit) << 23);
+        *scale = (stride ? 1.f : *dloss) * (mean ? 1.f / fmaxf(totals[2], 1.f) : 1.f) * __uint_as_float((unsigned)(127 + unit) << 23);
 }
 
-// ---- e of a piece -> its dz, 64 rows x 256 classes a workgroup; dbp [row blocks][ld]: the columns' sums over the 64 rows
-template <int PL>
+// ---- e of a piece -> its dz, ROWS rows x 256 classes a workgroup; dbp [row blocks][ld]: the columns' sums over its rows.  64 rows
+// a workgroup, 16 where that would leave the chip idle.
+template <int PL, int ROWS>
 __global__ __launch_bounds__(256) void xe_dz_kernel(const void* __restrict__ E, long long lde, long long e0,
                                                     const float* __restrict__ tmax, const float* __restrict__ lse,
                                                     const float* __restrict__ zlab, const float* __restrict__ rowg,
                                                     const long long* __restrict__ labels, long long M, long long v0,
                                                     short* __restrict__ dz, long long ld, float* __restrict__ dbp) {
-    __shared__ float f[64], at_label[64];
-    __shared__ int own[64];
+    __shared__ float f[ROWS], at_label[ROWS];
+    __shared__ int own[ROWS];
     __shared__ float sums[8][XT];
-    const long long m0 = (long long)blockIdx.y * 64, n0 = (long long)blockIdx.x * XT;
-    if (threadIdx.x < 64) {
+    const long long m0 = (long long)blockIdx.y * ROWS, n0 = (long long)blockIdx.x * XT;
+    if (threadIdx.x < ROWS) {
         const long long m = m0 + threadIdx.x;
         const float g = m < M ? rowg[m] : 0.f;
         const float mx = m < M ? tmax[(v0 / XT + blockIdx.x) * M + m] : 0.f;
@@ -483,7 +486,7 @@ __global__ __launch_bounds__(256) void xe_dz_kernel(const void* __restrict__ E, 
     const int cl = (threadIdx.x & 31) * 8, rl = threadIdx.x >> 5;
     float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < ROWS / 8; ++i) {
         const int r = rl + i * 8;
         const long long m = m0 + r;
         if (m >= M) continue;
@@ -555,7 +558,7 @@ template <int PL, int LN, int WL, int WR>
 __global__ __launch_bounds__(64 * WL * WR) void xe_dx_kernel(const short* __restrict__ dz, long long ldz, const short* __restrict__ W,
                                                              long long ldw, long long w_left, long long M, long long K, int blocks,
                                                              int splits, int accumulate, float* __restrict__ slab, long long ldk) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false> G;
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false, LN == 64 ? 3 : 2> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long nrow = (M + LN - 1) / LN, ncol = (K + XT - 1) / XT, tiles = nrow * ncol;
     auto job_at = [&](long long t, long long& m0, long long& k0, int& split) {
@@ -608,6 +611,7 @@ __global__ __launch_bounds__(256) void xe_dx_finish_kernel(const float* __restri
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < M * K; i += (long long)gridDim.x * 256) {
         const long long m = i / K, k = i - m * K;
         float s = 0.f;
+#pragma unroll 8
         for (int p = 0; p < splits; ++p) s += slab[((long long)p * M + m) * ldk + k];
         xe_put(DX + i, s * iw * g);
     }
@@ -765,14 +769,14 @@ struct BwdBuffers {
         slab = c.take<float>(p.splits * p.M * p.ldk);
         rowg = c.take<float>(p.M);
         scale = c.take<float>(1);
-        dbp = c.take<float>((p.M + 63) / 64 * p.piece);
+        dbp = c.take<float>((p.M + 15) / 16 * p.piece);
         bytes = c.used;
     }
     long long bytes;
 };
 
-// One workgroup a compute unit where the tiles take most of its LDS, two where they take half.
-unsigned grid_for(long long items, int lds) { return (unsigned)lowest(items, lds > (80 << 10) ? 256 : 512); }
+// One workgroup a compute unit: the stages take most of its LDS.
+unsigned grid_for(long long items) { return (unsigned)lowest(items, 256); }
 
 template <typename F>
 int with_lds(F* kernel, int bytes) {
@@ -816,6 +820,14 @@ int piece_of_w(const Plan& p, const void* W, long long v0, long long cols, short
     return pack(p, src, p.V, p.K, cols, buf, p.ldw, nullptr, 0, nullptr, amax + 1, stream);
 }
 
+// What a forward pass leaves for the backward pass, in one block of floats.
+struct State {
+    float *lse, *zlab, *totals, *tmax;
+    unsigned* amax;
+    State(float* base, long long M)
+        : lse(base), zlab(base + M), totals(base + 2 * M), tmax(base + 2 * M + 6), amax(reinterpret_cast<unsigned*>(base + 2 * M + 4)) {}
+};
+
 struct Call {
     const void *X, *W, *B;
     const long long* labels;
@@ -827,12 +839,12 @@ template <int PL, int LN, int WL, int WR>
 int launch_logits(const Plan& p, const Call& c, const short* x, const short* w, long long left, long long v0, long long vend,
                   const unsigned* amax, float* tmax, float* tsum, float* zlab, float* beaten, void* E, long long lde, long long e0,
                   long long e_tiles) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true> G;
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, true, LN == 64 ? 3 : 2> G;
     auto* kernel = &xe_logits_kernel<PL, LN, WL, WR>;
     constexpr int lds = G::LDS_BYTES + (XT + 2 * WR * LN + 2 * LN) * 4;
     XE_TRY(with_lds(kernel, lds));
     const long long tiles = ((p.M + LN - 1) / LN) * ((vend - v0 + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles, lds)), dim3(G::THREADS), lds, c.stream, x, p.ldx, w, p.ldw, left, c.B,
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(G::THREADS), lds, c.stream, x, p.ldx, w, p.ldw, left, c.B,
                        p.type, c.labels, p.M, p.K, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
     DTF_CHECK_LAUNCH();
     return 0;
@@ -850,12 +862,12 @@ int logits(const Plan& p, const Call& c, const short* x, const short* w, long lo
 
 template <int PL, int LN, int WL, int WR>
 int launch_dx(const Plan& p, const short* dz, const short* w, long long left, long long cols, int first, float* slab, hipStream_t stream) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false> G;
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, false, false, LN == 64 ? 3 : 2> G;
     auto* kernel = &xe_dx_kernel<PL, LN, WL, WR>;
     XE_TRY(with_lds(kernel, G::LDS_BYTES));
     const long long tiles = ((p.M + LN - 1) / LN) * ((p.K + XT - 1) / XT);
     const int blocks = (int)((cols + G::CB - 1) / G::CB), splits = (int)lowest(p.splits, blocks);   // (a last piece may be short)
-    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles * splits, G::LDS_BYTES)), dim3(G::THREADS), G::LDS_BYTES, stream, dz, p.piece * PL, w,
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles * splits)), dim3(G::THREADS), G::LDS_BYTES, stream, dz, p.piece * PL, w,
                        p.ldw, left, p.M, p.K, blocks, splits, !first, slab, p.ldk);
     DTF_CHECK_LAUNCH();
     return 0;
@@ -868,15 +880,17 @@ int launch_dw(const Plan& p, const short* x, const short* dz, long long v0, long
     auto* kernel = &xe_dw_kernel<PL, OUT_BF16>;
     XE_TRY(with_lds(kernel, G::LDS_BYTES));
     const long long tiles = ((p.K + 255) / 256) * ((cols + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles, G::LDS_BYTES)), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
                        cols, amax, scale, DW, p.V, v0);
     DTF_CHECK_LAUNCH();
     return 0;
 }
 
-int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, float* tmax, float* totals, unsigned* amax, void* kept,
-            long long kept_cols, void* ws) {
+int forward(const Plan& p, const Call& c, float* loss, const State& st, void* kept, long long kept_cols, int reduction, float* reduced,
+            void* ws) {
     const FwdBuffers b(p, ws);
+    float *tmax = st.tmax, *zlab = st.zlab;
+    unsigned* amax = st.amax;
     if (p.pl == 2) {
         hipLaunchKernelGGL(xe_amax_kernel, dim3(XE_AMAX), dim3(256), 0, c.stream, static_cast<const float*>(c.X), p.M, p.K, c.labels,
                            c.ignore, static_cast<const float*>(c.W), p.K * p.V, b.partial);
@@ -895,21 +909,27 @@ int forward(const Plan& p, const Call& c, float* loss, float* lse, float* zlab, 
     int rows = 16;
     while (rows > 1 && rows / 2 >= p.M) rows /= 2;
     hipLaunchKernelGGL(xe_merge_kernel, dim3((unsigned)((p.M + rows - 1) / rows)), dim3(256), 0, c.stream, tmax, b.tsum, p.tiles,
-                       c.labels, p.M, p.V, c.ignore, rows, zlab, b.beaten, lse, loss, b.hit);
+                       c.labels, p.M, p.V, c.ignore, rows, zlab, b.beaten, st.lse, loss, b.hit);
     DTF_CHECK_LAUNCH();
-    hipLaunchKernelGGL(xe_total_kernel, dim3(1), dim3(1024), 0, c.stream, loss, b.hit, c.labels, p.M, c.ignore, totals);
-    DTF_CHECK_LAUNCH();
+    if (reduction) {
+        hipLaunchKernelGGL(xe_total_kernel, dim3(1), dim3(1024), 0, c.stream, loss, b.hit, c.labels, p.M, c.ignore, st.totals, reduction,
+                           reduced);
+        DTF_CHECK_LAUNCH();
+    }
     return 0;
 }
 
-int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, float* tmax, const float* totals, unsigned* amax,
-             const void* kept, long long kept_cols, int mean, const float* dloss, int stride, void* DX, void* DW, void* DB, void* ws) {
+int backward(const Plan& p, const Call& c, const State& st, const void* kept, long long kept_cols, int mean, const float* dloss, int stride,
+             void* DX, void* DW, void* DB, void* ws) {
     const BwdBuffers b(p, ws);
+    float *tmax = st.tmax, *zlab = st.zlab, *lse = st.lse, *totals = st.totals;
+    unsigned* amax = st.amax;
     hipLaunchKernelGGL(xe_weights_kernel, dim3(1), dim3(1024), 0, c.stream, dloss, stride, totals, mean, c.labels, p.M, p.V, c.ignore,
                        lse, zlab, b.rowg, b.scale);
     DTF_CHECK_LAUNCH();
     if (DW || kept_cols < p.V) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, nullptr, amax, c.stream));
-    const long long rowblocks = (p.M + 63) / 64;
+    const int dz_rows = (p.M + 63) / 64 * ((p.piece + XT - 1) / XT) < 1024 ? 16 : 64;
+    const long long rowblocks = (p.M + dz_rows - 1) / dz_rows;
     for (long long v0 = 0; v0 < p.V; v0 += p.piece) {
         const long long cols = lowest(p.piece, p.V - v0), ct = (cols + XT - 1) / XT;
         const short* w = nullptr;
@@ -930,12 +950,10 @@ int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, 
             short* dz = b.dz + t0 * XT * p.pl;
             float* sums = dbp ? dbp + t0 * XT : nullptr;
             const dim3 grid((unsigned)(t1 - t0), (unsigned)rowblocks);
-            if (p.pl == 1)
-                hipLaunchKernelGGL(xe_dz_kernel<1>, grid, dim3(256), 0, c.stream, e, lde, e0, tmax, lse, zlab, b.rowg, c.labels, p.M, at,
-                                   dz, p.piece, sums);
-            else
-                hipLaunchKernelGGL(xe_dz_kernel<2>, grid, dim3(256), 0, c.stream, e, lde, e0, tmax, lse, zlab, b.rowg, c.labels, p.M, at,
-                                   dz, p.piece * 2, sums);
+            auto* kernel = p.pl == 1 ? (dz_rows == 16 ? &xe_dz_kernel<1, 16> : &xe_dz_kernel<1, 64>)
+                                     : (dz_rows == 16 ? &xe_dz_kernel<2, 16> : &xe_dz_kernel<2, 64>);
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, c.stream, e, lde, e0, tmax, lse, zlab, b.rowg, c.labels, p.M, at, dz,
+                               p.piece * p.pl, sums);
             DTF_CHECK_LAUNCH();
         }
         if (DX) {
@@ -980,12 +998,12 @@ int backward(const Plan& p, const Call& c, const float* lse, const float* zlab, 
 }
 
 bool sizes_ok(long long M, long long K, long long V, int type) {
-    return M > 0 && K > 0 && V > 0 && (type == 0 || type == 1) && M <= 65535ll * 64 && K <= (1ll << 20) && V <= (1ll << 22);
+    return M > 0 && K > 0 && V > 0 && (type == 0 || type == 1) && M <= 65535ll * 16 && K <= (1ll << 20) && V <= (1ll << 22);
 }
 
 }  // namespace
 
-// The largest sizes: 4194240 rows, 1048576 features, 4194304 classes (32-bit offsets within a tile; rows in blocks of 64 as
+// The largest sizes: 1048560 rows, 1048576 features, 4194304 classes (32-bit offsets within a tile; rows in blocks of 16 as
 // the second grid dimension).
 DTF_API int dtf_linear_xent_supported(long long M, long long K, long long V) { return sizes_ok(M, K, V, 0) ? 1 : 0; }
 
@@ -996,27 +1014,29 @@ DTF_API long long dtf_linear_xent_bwd_workspace_bytes(const void* W, long long M
     return sizes_ok(M, K, V, type) ? BwdBuffers(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;
 }
 
+// floats of the state between the two passes
+DTF_API long long dtf_linear_xent_state_floats(long long M, long long V) { return 2 * M + 6 + (V + XT - 1) / XT * M; }
+
 // type: 0 fp32, 1 bf16 (x, w, b alike; b may be null).  bf16 != 0: fp32 operands rounded to bf16 for the products.
-// loss, lse, zlab: M floats each; tmax: M floats for every 256 classes; totals: 4 floats (sum, counted rows, mean, rows whose
-// label has the largest logit); amax: 2 words (fp32 products only).  kept (may be null): [M, kept_cols] fp32 - bf16 where the
-// products take bf16 -, kept_cols a multiple of 256.
+// loss: M floats.  state: [2 M, 2 M + 4) holds the sum of the losses, the rows whose label has the largest logit, the counted
+// rows and the mean, if reduction is not 0; reduced (may be null): the mean (reduction 1) or the sum (2).  kept (may be null):
+// [M, kept_cols] fp32 - bf16 where the products take bf16 -, kept_cols a multiple of 256.
 DTF_API int dtf_linear_xent_fwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
-                                long long V, int type, int bf16, long long ignore, float* loss, float* lse, float* zlab, float* tmax,
-                                float* totals, unsigned* amax, void* kept, long long kept_cols, void* workspace, hipStream_t stream) {
+                                long long V, int type, int bf16, long long ignore, float* loss, float* state, void* kept,
+                                long long kept_cols, int reduction, float* reduced, void* workspace, hipStream_t stream) {
     if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
     const Call c = {X, W, B, labels, ignore, stream};
-    return forward(make_plan(W, M, K, V, type, bf16), c, loss, lse, zlab, tmax, totals, amax, kept, kept ? kept_cols : 0, workspace);
+    return forward(make_plan(W, M, K, V, type, bf16), c, loss, State(state, M), kept, kept ? kept_cols : 0, reduction, reduced, workspace);
 }
 
 // dloss: the loss's gradient, one float for all rows (stride 0) or one a row (stride 1); mean != 0: divided by the counted
-// rows.  DX, DW, DB may each be null.
+// rows (the forward pass had a reduction).  DX, DW, DB may each be null.
 DTF_API int dtf_linear_xent_bwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
-                                long long V, int type, int bf16, long long ignore, const float* lse, const float* zlab, float* tmax,
-                                const float* totals, unsigned* amax, const void* kept, long long kept_cols, int mean,
-                                const float* dloss, int dloss_stride, void* DX, void* DW, void* DB, void* workspace,
+                                long long V, int type, int bf16, long long ignore, float* state, const void* kept, long long kept_cols,
+                                int mean, const float* dloss, int dloss_stride, void* DX, void* DW, void* DB, void* workspace,
                                 hipStream_t stream) {
     if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
     const Call c = {X, W, B, labels, ignore, stream};
-    return backward(make_plan(W, M, K, V, type, bf16), c, lse, zlab, tmax, totals, amax, kept, kept ? kept_cols : 0, mean, dloss,
-                    dloss_stride, DX, DW, DB, workspace);
+    return backward(make_plan(W, M, K, V, type, bf16), c, State(state, M), kept, kept ? kept_cols : 0, mean, dloss, dloss_stride, DX, DW,
+                    DB, workspace);
 }

@@ -140,19 +140,17 @@ class _LinearXentFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, b, labels, ignore_index, reduction, bf16):
-        loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16, keep=any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, w, b, labels, *state)
+        loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16, True, reduction)
+        ctx.save_for_backward(x, w, b, labels, state.block, state.kept)
         ctx.cfg = (ignore_index, reduction, bf16)
-        if reduction == "none":
-            return loss
-        return state.totals[2 if reduction == "mean" else 0].clone()
+        return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
         x, w, b, labels = ctx.saved_tensors[:4]
-        state = F.LinearXentState(*ctx.saved_tensors[4:])
         ignore_index, reduction, bf16 = ctx.cfg
+        state = F.LinearXentState(*ctx.saved_tensors[4:], reduction)
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
         dw = torch.empty_like(w) if need[1] else None
@@ -171,9 +169,13 @@ def linear_softmax_cross_entropy(x, w, labels, b=None, ignore_index: int = -1, r
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     if tuple(labels.shape) != tuple(x.shape[:-1]):
         raise ValueError("labels %s do not fit x %s" % (tuple(labels.shape), tuple(x.shape)))
-    c = lambda t: None if t is None else t.contiguous()
-    loss = _LinearXentFn.apply(c(x.reshape(-1, x.shape[-1])), c(w), c(b), c(labels.reshape(-1).to(torch.int64)),
-                               int(ignore_index), reduction, bool(bf16))
+    c = lambda t: t if t is None or t.is_contiguous() else t.contiguous()
+    rows = c(labels.to(torch.int64).reshape(-1))
+    x, w, b = c(x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x), c(w), c(b)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+        loss = _LinearXentFn.apply(x, w, b, rows, int(ignore_index), reduction, bool(bf16))
+    else:
+        loss = F.linear_xent_forward(x, w, b, rows, int(ignore_index), bool(bf16), False, reduction)[0]
     return loss.reshape(labels.shape) if reduction == "none" else loss
 
 

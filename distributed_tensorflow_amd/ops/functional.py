@@ -576,9 +576,10 @@ def softmax_xent(z, labels, grad_out=None, grad_scale=None, stats=None):
 
 # --------------------------------------------------------------------------- softmax cross-entropy over a large vocabulary
 _XENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
-#: what ``linear_xent_forward`` leaves for ``linear_xent_backward``.  ``totals``: sum of the losses, counted rows, their mean,
-#: rows whose label has the largest logit (ties go to the lowest class); ``kept``: exponentials of the first logits or None
-LinearXentState = collections.namedtuple("LinearXentState", ["lse", "label_logit", "totals", "tile_max", "scales", "kept"])
+#: what ``linear_xent_forward`` leaves for ``linear_xent_backward``: every row's logsumexp, its label's logit, the totals and
+#: what else the kernels need, in one block of floats; the exponentials of the first logits, or None; the reduction
+LinearXentState = collections.namedtuple("LinearXentState", ["block", "kept", "reduction"])
+_XENT_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 #: bytes of exponentials that a forward pass with ``keep=True`` may leave for its backward pass (1/288 of an MI355X's memory)
 LINEAR_XENT_KEEP_BYTES = 1 << 30
 _XENT_TILE = 256
@@ -597,8 +598,8 @@ def _linear_xent_check(x, w, b, labels):
     for t in (x, w, b, labels):
         if t is not None and (t.device != x.device or not t.is_contiguous()):
             raise ValueError("x, w, b and labels must be contiguous and on one device")
-    if x.shape[0] > 4194240 or x.shape[1] > (1 << 20) or w.shape[1] > (1 << 22):
-        raise ValueError("at most 4194240 rows, 1048576 features and 4194304 classes, got %s, %s" % (tuple(x.shape), tuple(w.shape)))
+    if x.shape[0] > 1048560 or x.shape[1] > (1 << 20) or w.shape[1] > (1 << 22):
+        raise ValueError("at most 1048560 rows, 1048576 features and 4194304 classes, got %s, %s" % (tuple(x.shape), tuple(w.shape)))
 
 
 def _linear_xent_logits(x, w, b, labels, ignore_index, bf16):
@@ -612,62 +613,83 @@ def _linear_xent_logits(x, w, b, labels, ignore_index, bf16):
     return x32, w32, z if b is None else z + b.float(), counted
 
 
-def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False):
+def linear_xent_totals(state, rows):
+    """Sum of the losses, number of rows whose label has the largest logit (ties go to the lowest class), number of counted
+    rows and mean loss (0 without a counted row) of a forward pass over ``rows`` rows with a reduction, as a float32 view."""
+    if state.reduction == "none":
+        raise ValueError("totals belong to a forward pass with a reduction")
+    return state.block[2 * rows:2 * rows + 4]
+
+
+def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False, reduction="mean"):
     """Softmax cross-entropy of the logits ``x @ w + b`` (x [M, K], w [K, V], b [V] or None; all float32 or all bfloat16)
     against int64 ``labels`` [M], for vocabularies whose [M, V] logits should not be in memory.
 
     Rows with the label ``ignore_index`` count for nothing, whatever x holds there; any other label outside ``[0, V)`` makes
-    its row's loss NaN.  Classes may be masked by a ``b`` of -infinity.  ``bf16=True``: float32 operands are rounded to
-    bfloat16 for the products.  Returns ``(loss [M] float32, state)``; the state is what ``linear_xent_backward`` needs.
+    its row's loss NaN.  Classes may be masked by a ``b`` of -infinity (their columns of w must be finite).  ``bf16=True``:
+    float32 operands are rounded to bfloat16 for the products.
 
-    ``keep=True`` (a backward pass will follow): up to ``LINEAR_XENT_KEEP_BYTES`` of the first classes' exponentials stay in
-    the state, which saves the backward pass their part of the product; it computes the others again, piece by piece."""
+    Returns ``(loss, state)``: the mean loss of the counted rows (0 without any) or their ``"sum"``, a float32 scalar, or with
+    ``reduction="none"`` every row's [M]; the state is what ``linear_xent_backward`` needs.  ``keep=True`` (a backward pass
+    will follow): up to ``LINEAR_XENT_KEEP_BYTES`` of the first classes' exponentials stay in the state, which saves the
+    backward pass their part of the product; it computes the others again, piece by piece."""
     _linear_xent_check(x, w, b, labels)
+    if reduction not in _XENT_REDUCTIONS:
+        raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     M, K, V = int(x.shape[0]), int(x.shape[1]), int(w.shape[1])
-    tiles = -(-V // _XENT_TILE)
-    new = lambda *n: torch.empty(n, dtype=torch.float32, device=x.device)
-    cols = 0
-    if keep and M and x.is_cuda:
-        size = 2 if bf16 or x.dtype == torch.bfloat16 else 4
-        cols = min(tiles, LINEAR_XENT_KEEP_BYTES // (M * size * _XENT_TILE)) * _XENT_TILE
-    kept = torch.empty((M, cols), dtype=torch.bfloat16 if size == 2 else torch.float32, device=x.device) if cols else None
-    loss, state = new(M), LinearXentState(new(M), new(M), new(4), new(tiles, M) if x.is_cuda else None, new(2), kept)
-    if M == 0:
-        state.totals.zero_()
-        return loss, state
-    if x.is_cuda:
+    rows = torch.empty(M, dtype=torch.float32, device=x.device)
+    reduced = torch.empty((), dtype=torch.float32, device=x.device) if reduction != "none" else None
+    if M and x.is_cuda:
         with nv.device_guard(x):
-            lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
-            ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(nv.ptr(w), M, K, V, t, int(bool(bf16)))),
-                             dtype=torch.uint8, device=x.device)
-            rc = lib.dtf_linear_xent_fwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
-                                         int(ignore_index), nv.ptr(loss), nv.ptr(state.lse), nv.ptr(state.label_logit),
-                                         nv.ptr(state.tile_max), nv.ptr(state.totals), nv.ptr(state.scales), nv.ptr(kept), cols,
-                                         nv.ptr(ws), nv.stream_ptr())
+            lib, t, bf16 = nv.kernels(), _XENT_TYPES[x.dtype], int(bool(bf16))
+            cols, kept = 0, None
+            if keep:
+                size = 2 if bf16 or t == 1 else 4
+                cols = min(-(-V // _XENT_TILE), LINEAR_XENT_KEEP_BYTES // (M * size * _XENT_TILE)) * _XENT_TILE
+            if cols:
+                kept = torch.empty((M, cols), dtype=torch.bfloat16 if size == 2 else torch.float32, device=x.device)
+            block = torch.empty(int(lib.dtf_linear_xent_state_floats(M, V)), dtype=torch.float32, device=x.device)
+            ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(nv.ptr(w), M, K, V, t, bf16)), dtype=torch.uint8,
+                             device=x.device)
+            rc = lib.dtf_linear_xent_fwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, bf16, int(ignore_index),
+                                         nv.ptr(rows), nv.ptr(block), nv.ptr(kept), cols, _XENT_REDUCTIONS[reduction],
+                                         nv.ptr(reduced), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_fwd")
-        return loss, state
-    _, _, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
-    state.lse.copy_(torch.logsumexp(z, dim=1))
-    valid = (labels >= 0) & (labels < V)
-    picked = z.gather(1, torch.where(valid, labels, torch.zeros_like(labels)).view(-1, 1)).view(-1)
-    state.label_logit.copy_(torch.where(valid, picked, torch.full_like(picked, float("nan"))))
-    loss.copy_(torch.where(counted, state.lse - state.label_logit, torch.zeros_like(loss)))
-    n = int(counted.sum())
-    hits = int((counted & valid & (z.argmax(dim=1) == labels)).sum())
-    state.totals.copy_(torch.tensor([float(loss.double().sum()), n, float(loss.double().sum()) / max(n, 1), hits]))
-    return loss, state
+        return rows if reduced is None else reduced, LinearXentState(block, kept, reduction)
+    block = torch.zeros(2 * M + 6, dtype=torch.float32, device=x.device)
+    if M:
+        _, _, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
+        valid = (labels >= 0) & (labels < V)
+        picked = z.gather(1, torch.where(valid, labels, torch.zeros_like(labels)).view(-1, 1)).view(-1)
+        block[:M] = torch.logsumexp(z, dim=1)
+        block[M:2 * M] = torch.where(valid, picked, torch.full_like(picked, float("nan")))
+        rows.copy_(torch.where(counted, block[:M] - block[M:2 * M], torch.zeros_like(rows)))
+        n = counted.sum()
+        hits = (counted & valid & (z.argmax(dim=1) == labels)).sum()
+        total = rows.double().sum()
+        block[2 * M:2 * M + 4] = torch.stack([total, hits.double(), n.double(), total / n.clamp(min=1)]).float()
+    if reduced is not None:
+        reduced.copy_(block[2 * M + (3 if reduction == "mean" else 0)])
+    return rows if reduced is None else reduced, LinearXentState(block, None, reduction)
 
 
 def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index=-1, bf16=False, dx=None, dw=None, db=None):
     """Gradient of ``linear_xent_forward`` into ``dx``, ``dw`` and ``db`` (like x, w and b; each may be None).
 
     ``dloss`` float32: the gradient of every row's loss [M], or one value for all of them; ``mean=True`` divides it by the
-    number of counted rows (the gradient of their mean loss, ``state.totals[2]``)."""
+    number of counted rows (the gradient of their mean loss)."""
     _linear_xent_check(x, w, b, labels)
     M, K, V = int(x.shape[0]), int(x.shape[1]), int(w.shape[1])
     if dloss.dtype != torch.float32 or dloss.device != x.device or not dloss.is_contiguous() or dloss.numel() not in (1, M) \
             or (dloss.numel() == 1) == (dloss.dim() == 1 and M != 1):
         raise ValueError("dloss must be float32 [%d], or a single value of no dimension" % M)
+    tiles = -(-V // _XENT_TILE) if x.is_cuda else 0
+    kept = state.kept
+    if state.block.numel() != 2 * M + 6 + tiles * M or state.block.device != x.device or (kept is not None and (
+            kept.shape[0] != M or kept.dtype != (torch.bfloat16 if bf16 or x.dtype == torch.bfloat16 else torch.float32))):
+        raise ValueError("state must be what linear_xent_forward returned for the same call")
+    if mean and state.reduction == "none":
+        raise ValueError("mean=True needs the state of a forward pass with a reduction")
     for name, t, like in (("dx", dx, x), ("dw", dw, w), ("db", db, b)):
         if t is not None and (like is None or t.dtype != like.dtype or t.shape != like.shape or t.device != x.device
                               or not t.is_contiguous()):
@@ -680,23 +702,22 @@ def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index
     if x.is_cuda:
         with nv.device_guard(x):
             lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
-            kept = state.kept
             ws = torch.empty(int(lib.dtf_linear_xent_bwd_workspace_bytes(nv.ptr(w), M, K, V, t, int(bool(bf16)))),
                              dtype=torch.uint8, device=x.device)
             rc = lib.dtf_linear_xent_bwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
-                                         int(ignore_index), nv.ptr(state.lse), nv.ptr(state.label_logit),
-                                         nv.ptr(state.tile_max), nv.ptr(state.totals), nv.ptr(state.scales), nv.ptr(kept),
+                                         int(ignore_index), nv.ptr(state.block), nv.ptr(kept),
                                          0 if kept is None else kept.shape[1], int(bool(mean)), nv.ptr(dloss),
                                          int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw), nv.ptr(db), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_bwd")
         return
     x32, w32, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
-    g = dloss.expand(M) / torch.clamp(state.totals[1], min=1.0) if mean else dloss.expand(M)
+    lse, label_logit = state.block[:M], state.block[M:2 * M]
+    g = dloss.expand(M) / torch.clamp(state.block[2 * M + 2], min=1.0) if mean else dloss.expand(M)
     valid = (labels >= 0) & (labels < V)
     g = torch.where(counted, torch.where(valid, g, torch.full_like(g, float("nan"))), torch.zeros_like(g))
-    dz = torch.exp(z - state.lse.view(-1, 1)) * g.view(-1, 1)
+    dz = torch.exp(z - lse.view(-1, 1)) * g.view(-1, 1)
     rows = torch.nonzero(valid).view(-1)
-    dz[rows, labels[rows]] = g[rows] * torch.expm1(state.label_logit[rows] - state.lse[rows])
+    dz[rows, labels[rows]] = g[rows] * torch.expm1(label_logit[rows] - lse[rows])
     dz = torch.where(counted.view(-1, 1), dz, torch.zeros_like(dz))
     if db is not None:
         db.copy_(dz.sum(dim=0))
