@@ -8,7 +8,8 @@
 // x, y, dy, dx are fp32, bf16 or fp16; gamma, beta, their gradients, all statistics and sums are fp32 or wider.  The mean is
 // kept as two floats: where a group has few channels, dgamma is what remains when sum du (x - mean) cancels, and a mean
 // rounded to one float would leave its rounding error times sum du there.  u is rounded after every operation (no fused
-// multiply-add), as the formula written out in separate operations is: next to relu's border both fall on one side.
+// multiply-add), as the formula written out in separate operations is, so that values within a rounding of relu's border seldom
+// fall on another side than there (one in some 1e8 does, with a gradient of its own in dx: no two ways of rounding agree on all).
 //
 // Everything is bound by memory.  A sample is one stream of S C values, read in vectors of 16 bytes at any alignment; a
 // workgroup takes T vectors a turn, T a multiple of C / gcd(C, vector): then a thread meets the same channels every turn and

@@ -386,7 +386,10 @@ def group_norm(x, gamma, beta, groups: int, eps: float = 1e-3, activation=None):
     """Differentiable ``activation(group_normalisation(x))`` over the last axis of a channels-last ``x`` [B, ..., C] (float32,
     bfloat16 or float16): the channels of every sample in ``groups`` groups, each over all its positions.  ``gamma`` /
     ``beta`` [C] may be None; ``activation``: None, 'relu', 'sigmoid', 'tanh' or 'silu'."""
-    return _GroupNormFn.apply(x.contiguous(), gamma, beta, int(groups), float(eps), F.groupnorm_activation(activation))
+    x, act = x.contiguous(), F.groupnorm_activation(activation)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gamma, beta)):
+        return _GroupNormFn.apply(x, gamma, beta, int(groups), float(eps), act)
+    return F.groupnorm_forward(x, _c(gamma), _c(beta), int(groups), float(eps), act)[0]
 
 
 def clip_grad_norm(parameters, max_norm: float):
