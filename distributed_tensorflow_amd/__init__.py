@@ -7,5 +7,5 @@ __version__ = "0.1.0"
 
 from . import callbacks, data, layers, losses, models, optimizers  # noqa: F401
 from .layers import (Activation, AveragePooling2D, BatchNormalization, Conv2D, Dense, Dropout, Flatten,  # noqa: F401
-                     GlobalAveragePooling2D, MaxPooling2D)
+                     GlobalAveragePooling2D, GroupNormalization, MaxPooling2D)
 from .models import Sequential  # noqa: F401

@@ -485,6 +485,7 @@ class GraphEngine(ModelEngine):
         if not getattr(model.strategy, "owns_optimizer_state", False):
             model.optimizer.create_slots(model.store)
         model.strategy.prepare(model)
+        _optimizers.require_whole_gradient(model.optimizer, model.strategy)
         model._extra_categorical = False
         model._report_binary = False
         model.matmul_dtype = "fp32"
@@ -959,6 +960,10 @@ class _BatchNormalization(_SymbolicLayerMixin, _layers.BatchNormalization):
     pass
 
 
+class _GroupNormalization(_SymbolicLayerMixin, _layers.GroupNormalization):
+    pass
+
+
 class _AveragePooling2D(_SymbolicLayerMixin, _layers.AveragePooling2D):
     pass
 
@@ -1001,6 +1006,7 @@ def _keras_bce(y_true, y_pred):
 keras = types.SimpleNamespace(
     layers=types.SimpleNamespace(Dense=_Dense, Dropout=_Dropout, Activation=_Activation, Flatten=_Flatten,
                                  Conv2D=_Conv2D, MaxPooling2D=_MaxPooling2D, BatchNormalization=_BatchNormalization,
+                                 GroupNormalization=_GroupNormalization,
                                  AveragePooling2D=_AveragePooling2D, GlobalAveragePooling2D=_GlobalAveragePooling2D),
     models=types.SimpleNamespace(Sequential=_Sequential),
     backend=_KerasBackend,

@@ -358,6 +358,68 @@ class BatchNormalization(Layer):
         return dx.view(dy.shape) if dx is not None else None
 
 
+class GroupNormalization(Layer):
+    """Keras' ``GroupNormalization(groups=32, axis=-1, epsilon=1e-3, center=True, scale=True)`` with an activation on top: every
+    sample's channels are normalised in ``groups`` groups of neighbours, each over all positions of the sample, in training and
+    inference alike (there are no moving averages).  ``activation``: None, 'relu', 'sigmoid', 'tanh' or 'silu'.  Works on
+    ``[B, C]`` and ``[B, H, W, C]``; variables ``gamma`` / ``beta``."""
+
+    prefix = "group_normalization"
+
+    def __init__(self, groups: int = 32, axis: int = -1, epsilon: float = 1e-3, center: bool = True, scale: bool = True,
+                 activation=None, name=None, input_shape=None):
+        super().__init__(name=name, input_shape=input_shape)
+        if axis not in (-1, 3, 1):
+            raise ValueError("GroupNormalization normalises the last axis (axis=-1)")
+        self.axis, self.groups, self.epsilon = axis, int(groups), float(epsilon)
+        self.center, self.scale = bool(center), bool(scale)
+        self.activation, self.act = activation, F.groupnorm_activation(activation)
+        self.gamma = self.beta = None
+        self._buf = _Buffers()
+        self._x = None
+
+    def get_config(self):
+        return {"class": "GroupNormalization", "name": self.name, "groups": self.groups, "axis": -1, "epsilon": self.epsilon,
+                "center": self.center, "scale": self.scale, "activation": self.activation}
+
+    def build(self, input_shape, store):
+        out = super().build(input_shape, store)
+        if self.axis != -1 and self.axis != len(input_shape):
+            raise ValueError("GroupNormalization normalises the last axis; got axis=%d for per-example shape %s"
+                             % (self.axis, tuple(input_shape)))
+        c = int(input_shape[-1])
+        if self.groups < 1 or c % self.groups:
+            raise ValueError("%d channels do not divide into %d groups" % (c, self.groups))
+        if self.scale:
+            self.gamma = store.create(self.name + "/gamma", (c,), "ones")
+        if self.center:
+            self.beta = store.create(self.name + "/beta", (c,), "zeros")
+        return out
+
+    @property
+    def variables(self):
+        return [v for v in (self.gamma, self.beta) if v is not None]
+
+    def _params(self):
+        return (self.gamma.tensor if self.gamma is not None else None), (self.beta.tensor if self.beta is not None else None)
+
+    def forward(self, x, training):
+        y = self._buf.get("y", x.shape, x.device)
+        stats = self._buf.get("stats", (3, x.shape[0], self.groups), x.device)
+        F.groupnorm_forward(x, *self._params(), self.groups, self.epsilon, self.act, out=y, stats=stats)
+        self._x = x
+        return y
+
+    def backward(self, dy):
+        x = self._x
+        dx = self._buf.get("dx", x.shape, x.device) if self.need_input_grad else None
+        F.groupnorm_backward(x, dy if dy.is_contiguous() else dy.contiguous(), *self._params(), self.groups,
+                             self._buf.get("stats", (3, x.shape[0], self.groups), x.device), self.act,
+                             self.gamma.grad if self.gamma is not None else None,
+                             self.beta.grad if self.beta is not None else None, dx)
+        return dx
+
+
 class Flatten(Layer):
     prefix = "flatten"
 
@@ -814,7 +876,7 @@ class GlobalAveragePooling2D(Layer):
 def layer_from_config(cfg: dict) -> Layer:
     """Rebuild a layer from its ``get_config()`` dictionary (``class`` names the layer type)."""
     classes = {c.__name__: c for c in (Dense, Dropout, Activation, Flatten, Conv2D, MaxPooling2D, BatchNormalization,
-                                       AveragePooling2D, GlobalAveragePooling2D)}
+                                       GroupNormalization, AveragePooling2D, GlobalAveragePooling2D)}
     kw = {k: v for k, v in cfg.items() if k != "class"}
     try:
         cls = classes[cfg["class"]]

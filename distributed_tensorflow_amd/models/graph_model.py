@@ -180,6 +180,10 @@ class GraphModel(Sequential):
             return A.batch_norm(x, self._leaf(layer.gamma) if layer.gamma is not None else None,
                                 self._leaf(layer.beta) if layer.beta is not None else None, layer.moving_mean.tensor,
                                 layer.moving_variance.tensor, layer.momentum, layer.epsilon, training)
+        if isinstance(layer, L.GroupNormalization):
+            return A.group_norm(x, self._leaf(layer.gamma) if layer.gamma is not None else None,
+                                self._leaf(layer.beta) if layer.beta is not None else None, layer.groups, layer.epsilon,
+                                layer.activation)
         raise NotImplementedError("layer %s is not supported in a graph model" % type(layer).__name__)
 
     def _eval(self, node, env: dict, training: bool):

@@ -60,11 +60,13 @@ class LocalStrategy:
 
     world_size = 1
     rank = 0
+    sees_whole_gradient = True
 
     def prepare(self, model):
         pass
 
     def apply_gradients(self, model):
+        model.optimizer.clip_gradients(model.store)
         model.optimizer.apply_and_finish(model.store)
 
     def reduce_stats(self, stats: torch.Tensor) -> torch.Tensor:
@@ -207,6 +209,7 @@ class Sequential:
         if not getattr(self.strategy, "owns_optimizer_state", False):
             self.optimizer.create_slots(self.store)      # (parameter-server workers hold none: their owners do)
         self.strategy.prepare(self)
+        optim_mod.require_whole_gradient(self.optimizer, self.strategy)
         # Keras rule: 'accuracy' with a non-crossentropy loss and output dim > 1 is categorical accuracy.
         self._extra_categorical = any(m in ("accuracy", "acc", "categorical_accuracy") for m in self.metrics) \
             and self.loss.primary_metric != "categorical"
@@ -282,6 +285,67 @@ class Sequential:
         self._tail_plan = (ia + 1, b, c)
         return self._tail_plan
 
+    # ------------------------------------------------------------------ wide softmax head
+    def wide_head(self, y: torch.Tensor):
+        """The softmax head of a model with more classes than the logits kernel takes, trained or scored with sparse softmax
+        cross-entropy on the GPU: the head's product and the loss then run together, without the logits in memory
+        (``csrc/kernels/linear_xent.hip``).  ``None`` otherwise."""
+        head = self._effective[-1] if self._effective else None
+        if not isinstance(head, Dense) or not head.emit_logits or head.act != ACT_NONE or head.fused_keep < 1.0 \
+                or head.units <= F.SOFTMAX_XENT_MAX_CLASSES or head is not self.layers[-1]:
+            return None
+        if self.device is None or self.device.type != "cuda" or y.dim() != 1 or y.dtype != torch.int64 \
+                or not isinstance(self.loss, losses_mod.SparseCategoricalCrossentropy):
+            return None
+        return head
+
+    def _wide_head_loss(self, head, x, y, stats, training: bool):
+        """Forward pass, loss and metrics; returns what the head's backward pass needs."""
+        h = x
+        for layer in self.layers[:-1]:
+            h = layer.forward(h, training)
+        bf16 = getattr(head, "matmul_dtype", "fp32") == "bf16"
+        _, state = F.linear_xent_forward(h, head.kernel.tensor, head.bias.tensor if head.bias is not None else None, y,
+                                         bf16=bf16, keep=training)
+        stats[:3].add_(F.linear_xent_totals(state, int(h.shape[0]))[:3])
+        return h, state, bf16
+
+    def _compute_gradients_wide_head(self, x, y, stats, head):
+        h, state, bf16 = self._wide_head_loss(head, x, y, stats, True)
+        one = self._grad_buf.get("one")
+        if one is None:
+            one = self._grad_buf["one"] = torch.ones((), dtype=torch.float32, device=h.device)
+        g = self._grad_like(h) if head.need_input_grad else None
+        bias = head.bias
+        F.linear_xent_backward(h, head.kernel.tensor, bias.tensor if bias is not None else None, y, state, one, True, bf16=bf16,
+                               dx=g, dw=head.kernel.grad, db=bias.grad if bias is not None else None)
+        if g is not None and head.fuse_prev_grad:      # the layer below hands its activation's gradient to this one
+            key = ("head dz", tuple(h.shape))
+            dz = self._grad_buf.get(key)
+            if dz is None:
+                dz = self._grad_buf[key] = torch.empty_like(h)
+            g = F.act_grad(g, h, head.prev_act, head.prev_scale, out=dz)
+        hook = self._after_layer_backward
+        if hook is not None:
+            hook(head, self)
+        for layer in reversed(self.layers[:-1]):
+            if g is None:
+                break
+            g = layer.backward(g)
+            if hook is not None:
+                hook(layer, self)
+
+    def _score(self, x, y, stats):
+        """Loss and metrics of a batch into ``stats``."""
+        head = self.wide_head(y)
+        if head is not None:
+            fresh = getattr(self.strategy, "ensure_fresh", None)
+            if fresh is not None:
+                fresh(self)
+            self._wide_head_loss(head, x, y.contiguous(), stats, False)
+        else:
+            self._loss_and_metrics(self.forward(x, training=False), y, False, stats)
+
     def _compute_gradients_tail(self, x, y, stats, plan):
         first, b, c = plan
         h = x
@@ -348,6 +412,9 @@ class Sequential:
         plan = self.tail_plan() if (x.is_cuda and y.dtype == torch.int64 and y.dim() == 1) else None
         if plan is not None:
             return self._compute_gradients_tail(x, y.contiguous(), self.stats if stats is None else stats, plan)
+        head = self.wide_head(y) if x.is_cuda else None
+        if head is not None:
+            return self._compute_gradients_wide_head(x, y.contiguous(), self.stats if stats is None else stats, head)
         out = self.forward(x, training=True)
         g = self._loss_and_metrics(out, y, True, self.stats if stats is None else stats)
         self.backward(g)
@@ -418,8 +485,7 @@ class Sequential:
         self._check_compiled()
         xb, yb = _as_tensor(x, self.device), _as_tensor(y, self.device)
         st = F.new_stats(self.device)
-        out = self.forward(xb, training=False)
-        self._loss_and_metrics(out, yb, False, st)
+        self._score(xb, yb, st)
         return self.read_stats(stats=st)
 
     def evaluate(self, x, y, batch_size: int = 32, verbose: int = 0) -> List[float]:
@@ -428,8 +494,7 @@ class Sequential:
         st = F.new_stats(self.device)
         n = xd.shape[0]
         for i in range(0, n, batch_size):
-            out = self.forward(xd[i:i + batch_size], training=False)
-            self._loss_and_metrics(out, yd[i:i + batch_size], False, st)
+            self._score(xd[i:i + batch_size], yd[i:i + batch_size], st)
         logs = self.read_stats(stats=self.strategy.reduce_stats(st))
         return [logs["loss"]] + ([logs["acc"]] if "acc" in logs else [])
 
@@ -529,6 +594,8 @@ class Sequential:
         if not isinstance(self.loss, losses_mod.MeanSquaredError):
             return None
         opt = self.optimizer
+        if opt.global_clipnorm is not None:
+            return None                     # the whole-step kernel updates each variable as its gradient is ready
         if isinstance(opt, optim_mod.Adam):
             kind = 0
             m, v = self.store.slot("m"), self.store.slot("v")

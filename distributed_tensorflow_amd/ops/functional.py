@@ -538,6 +538,10 @@ def bce_loss(p, y, grad_out=None, grad_scale=None, through_sigmoid=False, stats=
     return grad_out
 
 
+#: classes that ``softmax_xent`` takes on the GPU with int64 labels (a workgroup stages 256 rows of logits in LDS)
+SOFTMAX_XENT_MAX_CLASSES = 149
+
+
 def softmax_xent(z, labels, grad_out=None, grad_scale=None, stats=None):
     """Softmax cross-entropy on logits ``z`` [M,C] + argmax accuracy, gradient fused.
 

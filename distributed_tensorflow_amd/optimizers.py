@@ -10,6 +10,10 @@ after a reduce-scatter) and "this owner's shard" (parameter-server owner).
 ``tf.train.*Optimizer`` or Keras' optimizer strings may name; each comes in the TensorFlow form (slot names, initial
 slot values and epsilon placement of TF's Apply* kernels, so checkpoints carry the names TF expects) and, through
 ``get('rmsprop')`` / ``get('adagrad')``, in the form of Keras 2.0.8's Python formulas.
+
+Every rule takes ``global_clipnorm``: the gradient of all variables together is clipped by its global norm before the update
+(``tf.clip_by_global_norm`` between ``compute_gradients`` and ``apply_gradients``).  That needs the whole gradient in one place:
+a single replica, or synchronous replicas that all-reduce it; other strategies refuse it.
 """
 from __future__ import annotations
 
@@ -23,6 +27,19 @@ class Optimizer:
     #: slot buffer name -> suffix used in TF checkpoints ("<var>/<suffix>")
     slot_checkpoint_names: Dict[str, str] = {}
     name = "optimizer"
+    #: Keras' ``global_clipnorm``: gradients are scaled down together so that their global norm is at most this; None: as they are
+    global_clipnorm: Optional[float] = None
+
+    def _set_clipnorm(self, value):
+        if value is not None and not float(value) > 0.0:
+            raise ValueError("global_clipnorm must be positive, got %r" % (value,))
+        self.global_clipnorm = None if value is None else float(value)
+
+    def clip_gradients(self, store: VariableStore, grad_scale: float = 1.0):
+        """Clip ``grad_scale`` times the whole flat gradient by its global norm, in place, where ``global_clipnorm`` asks for it.
+        (The flat buffer's alignment gaps are zeros and count for nothing.)"""
+        if self.global_clipnorm is not None:
+            F.clip_by_global_norm([store.flat_grad], self.global_clipnorm / grad_scale, out=[store.flat_grad])
 
     @property
     def slot_order(self):
@@ -65,7 +82,8 @@ class Adam(Optimizer):
 
     def __init__(self, lr: float = 1e-3, beta_1: float = 0.9, beta_2: float = 0.999, epsilon: float = 1e-8,
                  learning_rate: Optional[float] = None, beta1: Optional[float] = None,
-                 beta2: Optional[float] = None):
+                 beta2: Optional[float] = None, global_clipnorm: Optional[float] = None):
+        self._set_clipnorm(global_clipnorm)
         self.lr = float(learning_rate if learning_rate is not None else lr)
         self.beta1 = float(beta1 if beta1 is not None else beta_1)
         self.beta2 = float(beta2 if beta2 is not None else beta_2)
@@ -106,7 +124,9 @@ class SGD(Optimizer):
     slot_checkpoint_names = {"momentum": "Momentum"}
     name = "SGD"
 
-    def __init__(self, lr: float = 0.01, momentum: float = 0.0, learning_rate: Optional[float] = None):
+    def __init__(self, lr: float = 0.01, momentum: float = 0.0, learning_rate: Optional[float] = None,
+                 global_clipnorm: Optional[float] = None):
+        self._set_clipnorm(global_clipnorm)
         self.lr = float(learning_rate if learning_rate is not None else lr)
         self.momentum = float(momentum)
 
@@ -145,7 +165,9 @@ class RMSProp(Optimizer):
     name = "RMSProp"
 
     def __init__(self, lr: float = 0.001, decay: float = 0.9, momentum: float = 0.0, epsilon: Optional[float] = None,
-                 learning_rate: Optional[float] = None, rho: Optional[float] = None, keras: bool = False):
+                 learning_rate: Optional[float] = None, rho: Optional[float] = None, keras: bool = False,
+                 global_clipnorm: Optional[float] = None):
+        self._set_clipnorm(global_clipnorm)
         self.lr = float(learning_rate if learning_rate is not None else lr)
         self.rho = float(rho if rho is not None else decay)
         self.momentum = float(momentum)
@@ -193,7 +215,8 @@ class Adagrad(Optimizer):
     name = "Adagrad"
 
     def __init__(self, lr: float = 0.01, initial_accumulator_value: Optional[float] = None, epsilon: Optional[float] = None,
-                 learning_rate: Optional[float] = None, keras: bool = False):
+                 learning_rate: Optional[float] = None, keras: bool = False, global_clipnorm: Optional[float] = None):
+        self._set_clipnorm(global_clipnorm)
         self.lr = float(learning_rate if learning_rate is not None else lr)
         self.keras = bool(keras)
         self.initial = float(initial_accumulator_value if initial_accumulator_value is not None else (0.0 if keras else 0.1))
@@ -231,7 +254,9 @@ class Adadelta(Optimizer):
     slot_checkpoint_names = {"accum": "Adadelta", "accum_update": "Adadelta_1"}
     name = "Adadelta"
 
-    def __init__(self, lr: float = 0.001, rho: float = 0.95, epsilon: float = 1e-8, learning_rate: Optional[float] = None):
+    def __init__(self, lr: float = 0.001, rho: float = 0.95, epsilon: float = 1e-8, learning_rate: Optional[float] = None,
+                 global_clipnorm: Optional[float] = None):
+        self._set_clipnorm(global_clipnorm)
         self.lr = float(learning_rate if learning_rate is not None else lr)
         self.rho, self.epsilon = float(rho), float(epsilon)
 
@@ -254,6 +279,14 @@ class Adadelta(Optimizer):
     def apply_and_finish(self, store, grad_scale=1.0):
         F.adadelta_apply(store.flat, store.slot("accum"), store.slot("accum_update"), store.flat_grad, self.lr, self.rho,
                          self.epsilon, grad_scale, advance=store.global_step)
+
+
+def require_whole_gradient(optimizer, strategy):
+    """Refuses ``global_clipnorm`` under a strategy whose updates never see the whole gradient (sharded synchronous replicas,
+    parameter servers)."""
+    if optimizer.global_clipnorm is not None and not getattr(strategy, "sees_whole_gradient", False):
+        raise ValueError("global_clipnorm needs the whole gradient in one place: a single replica, or synchronous replicas of a model "
+                         "small enough to be all-reduced; %s updates parts of it" % type(strategy).__name__)
 
 
 def from_description(desc: dict) -> Optimizer:

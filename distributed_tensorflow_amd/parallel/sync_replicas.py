@@ -232,6 +232,10 @@ class SyncReplicasStrategy:
         self._comm_pending = keep
         return self._comm_total
 
+    @property
+    def sees_whole_gradient(self) -> bool:
+        return self.replicated
+
     def _apply_replicated(self, model, scale):
         store = model.store
         c = self.comm
@@ -258,6 +262,7 @@ class SyncReplicasStrategy:
             if work is not None and hasattr(work, "wait"):
                 work.wait()            # stream-level wait under RCCL: the host does not block
         self._comm_end(store, t_comm)
+        model.optimizer.clip_gradients(store, grad_scale=scale)
         model.optimizer.apply_and_finish(store, grad_scale=scale)
 
     def apply_gradients(self, model):
