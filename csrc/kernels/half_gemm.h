@@ -20,7 +20,7 @@
 //
 // LDS layouts.  RC: row of 128 bytes = 8 chunks of 16; chunk c of row i lies at c ^ ((i >> 1) & 7): LDS delivers 256 bytes a
 // cycle, 16 lanes of a fragment read, whose 16 rows at one c are then on 16 different chunks of two rows' width (with i & 7
-// every second chunk would be hit twice: measured as one conflict cycle for each useful one).  RS: row k of LN * PL halves in granules of 32 bytes; granule q of
+// every second chunk would be hit twice: measured as one conflict cycle for each useful one).  RS: row k of N * PL halves in granules of 32 bytes; granule q of
 // row k lies at q ^ 2 (k & 3): a transposing read takes 4 rows x 2 granules at once, which are then 8 distinct ones of 256 bytes.
 // The direct load writes LDS linearly, so the permutation is applied to the addresses it loads from.
 #pragma once
@@ -98,11 +98,18 @@ struct Gemm {
     static constexpr int LOADS = (LN + RN) / 8 / WAVES;      // a wave and stage, 1 KB each
     static constexpr int KS = CB / 16;                       // MFMA steps a stage and limb product
     static_assert(LN % (32 * WL) == 0 && RN % (32 * WR) == 0 && (LN / 8) % WAVES == 0 && (RN / 8) % WAVES == 0, "tile");
-    static_assert((!L_RS || LN == 256) && (!R_RS || RN == 256), "the RS layout's banks are worked out for rows of 256 values");
+    static_assert((!L_RS || LN == 256 || LN == 64) && (!R_RS || RN == 256), "the RS layout's banks are worked out for these rows");
 
     static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const char* base, long long left) {
         const long long n = left < 0 ? 0 : left > 0xffffffffll ? 0xffffffffll : left;
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, (int)(unsigned)n, 0x00020000);
+    }
+
+    // granule permutation of row k of an RS tile of N values: 4 rows by 2 granules on 8 granules of 256 bytes; rows of 128 bytes
+    // (64 values, one limb) lie two to 256 bytes
+    template <int N>
+    static __device__ __forceinline__ int rs_swap(int k) {
+        return N * PL == 64 ? k & 2 : 2 * (k & 3);
     }
 
     // LDS <- stage `blk` of one operand
@@ -123,18 +130,18 @@ struct Gemm {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
                                                          (int)(row0 + 8 * i * ld + (i & 1 ? chunk ^ 64 : chunk)), 0, 0, 0);
         } else {
-            constexpr int SLOTS = N * PL / 8;                // 16-byte chunks a row: 32 or 64
-            constexpr int ROWS = 64 / SLOTS;                 // rows a load: 2 or 1
+            constexpr int SLOTS = N * PL / 8;                // 16-byte chunks a row: 8 to 64
+            constexpr int ROWS = 64 / SLOTS;                 // rows a load: 8 to 1
             const long long skip = (long long)blk * CB * t.ld;
             const __amdgpu_buffer_rsrc_t rs = resource(t.base + skip, t.left - skip);
             const unsigned ld = (unsigned)t.ld;
             static_assert(LOADS * ROWS % 4 == 0, "a wave's first row is a multiple of 4");
             const unsigned row0 = (unsigned)(wave * LOADS * ROWS + lane / SLOTS) * ld;
-            const unsigned chunk = (unsigned)((lane % SLOTS) ^ (4 * (lane / SLOTS))) * 16;
+            const unsigned chunk = (unsigned)((lane % SLOTS) ^ (2 * rs_swap<N>(lane / SLOTS))) * 16;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + (wave * LOADS + i) * 1024), 16,
-                                                         (int)(row0 + ROWS * i * ld + (chunk ^ (64 * (ROWS * i & 3)))), 0, 0, 0);
+                                                         (int)(row0 + ROWS * i * ld + (chunk ^ (32 * rs_swap<N>(ROWS * i)))), 0, 0, 0);
         }
     }
 
@@ -149,7 +156,7 @@ struct Gemm {
         constexpr int ROW = N * PL * 2;
         const int granule = tile32 * 2 * PL + plane * 2 + ((lane >> 4) & 1);
         const int row = kk * 16 + (lane >> 5) * 8 + ((lane >> 2) & 3);
-        const lds_char* p = src + row * ROW + ((granule ^ (2 * ((lane >> 2) & 3))) * 32) + (lane & 3) * 8;
+        const lds_char* p = src + row * ROW + ((granule ^ rs_swap<N>((lane >> 2) & 3)) * 32) + (lane & 3) * 8;
         const s16x4 lo = read_tr(p), hi = read_tr(p + 4 * ROW);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
@@ -224,7 +231,8 @@ struct Gemm {
     }
 
     // Tiles of few rows: so little to multiply that a stage takes as long as its loads' way, so STAGES - 1 stages are on their way at
-    // a time (128 rows, 512 features, 10001 classes, fp32: @SMALL@).  The loads of stages behind the last
+    // a time.  64 rows against 128 tiles of columns, 4096 features, two stages / three: fp32 156 / 112 us, bf16 60 / 51 us (5.3 TB/s);
+    // 512 features: 16.6 / 16.0 and 8.3 / 8.7 us; four stages are no faster than three.  The loads of stages behind the last
     // one are issued all the same, out of bounds, so that the number in flight is a constant.
     static __device__ __forceinline__ void ring(const Job& job, int wl, int wr, lds_char* smem, f32x16 (&acc)[TL][TR]) {
         const Tile none_l = {job.l.base, 0, job.l.ld}, none_r = {job.r.base, 0, job.r.ld};
@@ -240,16 +248,18 @@ struct Gemm {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * LOADS) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            issue(blk + STAGES - 1, ahead);
+            Frags f[KS];                                     // one wave a SIMD: all reads of a stage first, not step by step
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                Frags f;
-                fetch(smem + now * STAGE, kk, wl, wr, f);
-                multiply(f, acc);
-            }
+            for (int kk = 0; kk < KS; ++kk) fetch(smem + now * STAGE, kk, wl, wr, f[kk]);
+            issue(blk + STAGES - 1, ahead);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) multiply(f[kk], acc);
+            __builtin_amdgcn_sched_barrier(0);
             now = now + 1 == STAGES ? 0 : now + 1;
             ahead = ahead + 1 == STAGES ? 0 : ahead + 1;
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // nothing is on its way into LDS when the workgroup ends
     }
 
     // Fragments a step ahead (8192 x 8192 x 2048: 1128 TFLOP/s where both operands are RC, against 1066 without; the others

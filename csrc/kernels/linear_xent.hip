@@ -618,19 +618,20 @@ __global__ __launch_bounds__(256) void xe_dx_finish_kernel(const float* __restri
 }
 
 // ---- dw[:, v0 ...] = x^T dz
-template <int PL, int OUT_BF16>
-__global__ __launch_bounds__(512) void xe_dw_kernel(const short* __restrict__ X, long long ldx, const short* __restrict__ dz, long long ldz,
+template <int PL, int OUT_BF16, int LN, int WL, int WR>
+__global__ __launch_bounds__(64 * WL * WR) void xe_dw_kernel(const short* __restrict__ X, long long ldx, const short* __restrict__ dz,
+                                                             long long ldz, long long dz_left,
                                                     long long M, long long K, long long cols, const unsigned* __restrict__ amax,
                                                     const float* __restrict__ scale, void* __restrict__ DW, long long V, long long v0) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, 256, XT, 2, 4, true, true> G;
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, true, true, LN == 64 ? 3 : 2> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    const long long nrow = (K + 255) / 256, ncol = (cols + XT - 1) / XT;
+    const long long nrow = (K + LN - 1) / LN, ncol = (cols + XT - 1) / XT;
     auto job_at = [&](long long t, long long& k0, long long& n0) {
         long long rt, ct;
         hgemm::tile_at(t, nrow, ncol, rt, ct);
-        k0 = rt * 256, n0 = ct * XT;
+        k0 = rt * LN, n0 = ct * XT;
         return typename G::Job{{reinterpret_cast<const char*>(X + k0 * PL), M * ldx * 2 - k0 * PL * 2, ldx * 2},
-                               {reinterpret_cast<const char*>(dz + n0 * PL), M * ldz * 2 - n0 * PL * 2, ldz * 2},
+                               {reinterpret_cast<const char*>(dz + n0 * PL), dz_left - n0 * PL * 2, ldz * 2},
                                (int)((M + G::CB - 1) / G::CB)};
     };
     const hgemm::Deal deal(nrow * ncol);
@@ -644,10 +645,10 @@ __global__ __launch_bounds__(512) void xe_dw_kernel(const short* __restrict__ X,
     G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
     const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) / XE_DZ_SCALE : 1.f;
     const float g = *scale;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / 4, wr = wave % 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
 #pragma unroll
     for (int a = 0; a < G::TL; ++a) {
-        const long long k = k0 + wl * 128 + a * 32 + (lane & 31);
+        const long long k = k0 + wl * (LN / WL) + a * 32 + (lane & 31);
         if (OUT_BF16) {
             short* out = static_cast<short*>(DW) + k * V + v0;
             const long long n = n0 + wr * 64 + 8 * (lane >> 5);
@@ -695,7 +696,7 @@ struct Plan {
     long long M, K, V;
     int type, pl;              // 0 fp32, 1 bf16 operands; limbs a value
     bool packs;                // w has to be packed
-    bool small;                // 64 rows a tile
+    bool small;                // 64 rows of x a tile
     long long ldx, ldw, piece, tiles;
     long long esize;
     int splits;                // of the classes of a piece for dx
@@ -719,11 +720,20 @@ Plan make_plan(const void* W, long long M, long long K, long long V, int type, i
     if (piece < XT) piece = XT;
     p.piece = lowest(piece, p.tiles * XT);
     p.ldw = p.packs ? p.piece * p.pl : V;
-    // enough workgroups for the chip from a product with few output tiles: the reduction over classes is split, eight stages
-    // at least a split
+    // dx has few output tiles for its long reduction, which is split: into as many parts as take the least time by the rounds of
+    // 256 workgroups that they need (1.3 us a stage) and the traffic of their sums (4.6 TB/s); eight stages at least a part.
+    // (2048 rows, 1024 features: 32 tiles -> 8 parts.)
     const long long out = ((M + (p.small ? 63 : 255)) / (p.small ? 64 : 256)) * ((K + XT - 1) / XT);
     const long long blocks = p.piece / cb;
-    p.splits = (int)lowest(lowest((256 + out - 1) / out, blocks / 8 > 0 ? blocks / 8 : 1), 64);
+    double best = 0.0;
+    p.splits = 1;
+    for (int s = 1; s <= 64 && s * 8 <= (blocks < 8 ? 8 : blocks); ++s) {
+        const double t = (double)((out * s + 255) / 256) / s * (double)blocks * 1.3e-6 + (double)s * M * K * 8 / 4.6e12;
+        if (s == 1 || t < best) {
+            best = t;
+            p.splits = s;
+        }
+    }
     p.ldk = up(K, 4);
     return p;
 }
@@ -853,11 +863,9 @@ int launch_logits(const Plan& p, const Call& c, const short* x, const short* w, 
 int logits(const Plan& p, const Call& c, const short* x, const short* w, long long left, long long v0, long long vend,
            const unsigned* amax, float* tmax, float* tsum, float* zlab, float* beaten, void* E, long long lde, long long e0,
            long long e_tiles) {
-    if (p.pl == 1)
-        return p.small ? launch_logits<1, 64, 1, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles)
-                       : launch_logits<1, 256, 2, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
-    return p.small ? launch_logits<2, 64, 1, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles)
-                   : launch_logits<2, 256, 2, 4>(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
+    auto* launch = p.pl == 1 ? (p.small ? &launch_logits<1, 64, 1, 4> : &launch_logits<1, 256, 2, 4>)
+                             : (p.small ? &launch_logits<2, 64, 1, 4> : &launch_logits<2, 256, 2, 4>);
+    return launch(p, c, x, w, left, v0, vend, amax, tmax, tsum, zlab, beaten, E, lde, e0, e_tiles);
 }
 
 template <int PL, int LN, int WL, int WR>
@@ -873,16 +881,37 @@ int launch_dx(const Plan& p, const short* dz, const short* w, long long left, lo
     return 0;
 }
 
+template <int PL, int OUT_BF16, int LN, int WL, int WR>
+int launch_dw_tiles(const Plan& p, const short* x, const short* dz, long long dz_left, long long v0, long long cols,
+                    const unsigned* amax, const float* scale, void* DW, hipStream_t stream) {
+    typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, true, true, LN == 64 ? 3 : 2> G;
+    auto* kernel = &xe_dw_kernel<PL, OUT_BF16, LN, WL, WR>;
+    XE_TRY(with_lds(kernel, G::LDS_BYTES));
+    const long long tiles = ((p.K + LN - 1) / LN) * ((cols + XT - 1) / XT);
+    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, dz_left,
+                       p.M, p.K, cols, amax, scale, DW, p.V, v0);
+    DTF_CHECK_LAUNCH();
+    return 0;
+}
+
+// dw's tiles of 256 x 256 go out in rounds of 256 workgroups.  What a last round holds goes to tiles of 64 rows if it is at most
+// half full: four times as many, a third of a round's time (50021 classes, 1024 features, 2048 rows: 241 + 39 us, and 297 us with
+// a last round of 16 tiles.  The logits gained nothing from it: 277 + 27 us for 301.)
+long long whole_columns(long long rows, long long cols) {
+    const long long nrow = (rows + 255) / 256, ncol = (cols + XT - 1) / XT;
+    if (rows <= 128) return 0;                                  // (64-row tiles waste less)
+    const long long whole = nrow * ncol / 256 * 256 / nrow;
+    return (ncol - whole) * nrow <= 128 ? whole : ncol;
+}
+
 template <int PL, int OUT_BF16>
 int launch_dw(const Plan& p, const short* x, const short* dz, long long v0, long long cols, const unsigned* amax, const float* scale,
               void* DW, hipStream_t stream) {
-    typedef Gemm<typename HalfOf<PL>::type, PL, 256, XT, 2, 4, true, true> G;
-    auto* kernel = &xe_dw_kernel<PL, OUT_BF16>;
-    XE_TRY(with_lds(kernel, G::LDS_BYTES));
-    const long long tiles = ((p.K + 255) / 256) * ((cols + XT - 1) / XT);
-    hipLaunchKernelGGL(kernel, dim3(grid_for(tiles)), dim3(G::THREADS), G::LDS_BYTES, stream, x, p.ldx, dz, p.piece * PL, p.M, p.K,
-                       cols, amax, scale, DW, p.V, v0);
-    DTF_CHECK_LAUNCH();
+    const long long done = lowest(whole_columns(p.K, cols) * XT, cols), left = p.M * p.piece * PL * 2;
+    if (done > 0) XE_TRY((launch_dw_tiles<PL, OUT_BF16, 256, 2, 4>(p, x, dz, left, v0, done, amax, scale, DW, stream)));
+    if (done < cols)
+        XE_TRY((launch_dw_tiles<PL, OUT_BF16, 64, 1, 4>(p, x, dz + done * PL, left - done * PL * 2, v0 + done, cols - done, amax, scale, DW,
+                                                        stream)));
     return 0;
 }
 

@@ -107,7 +107,8 @@ def test_loss_and_gradients(device, dtype, size):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("size", [(1, 512, 32001), (17, 1000, 4096), (257, 72, 12345), (300, 520, 2049), (1024, 256, 8192),
-                                  (2047, 128, 33000), (9000, 64, 4097), (33, 2056, 8200)])
+                                  (2047, 128, 33000), (9000, 64, 4097), (33, 2056, 8200),
+                                  (1500, 1100, 12000), (700, 260, 40000), (2100, 520, 8000)])
 def test_loss_and_gradients_of_larger_sizes(gpu_device, dtype, size):
     _check(*_inputs(*size, dtype, "cuda", bias=size[1] != 72), reduction=["mean", "none"][size[2] % 2])
 
