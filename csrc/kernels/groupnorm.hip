@@ -864,12 +864,12 @@ int grp_bwd(const Args& a, const void* X, const void* DY, void* DX, const float*
 
 bool grp_ok(long long B, long long S, int C, int G, int type, int act) {
     return B > 0 && S > 0 && C > 0 && G > 0 && C % G == 0 && type >= 0 && type <= 2 && act >= ACT_NONE && act <= ACT_SILU &&
-           C <= (1 << 20) && B <= (1 << 21);
+           C <= (1 << 20) && G <= (1 << 14) && B <= (1 << 21);
 }
 
 }  // namespace
 
-// At most 2097152 samples (a grid's threads are counted in 32 bits) and 1048576 channels.
+// At most 2097152 samples (a grid's threads are counted in 32 bits), 1048576 channels and 16384 groups (their means stand in LDS).
 // doubles of scratch that a call needs, either direction
 DTF_API long long dtf_groupnorm_workspace_doubles(long long B, long long S, int C, int type) {
     const Plan p = make_plan(B, S, C, type ? 2 : 4);

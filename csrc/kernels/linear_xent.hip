@@ -13,11 +13,12 @@
 //
 // Numbers.  bf16 operands multiply as they are.  fp32 operands are scaled by a power of two for each tensor (largest value
 // in [2^14, 2^15)) and split into two fp16 limbs of 22 bits together, multiplied as three limb products (half_gemm.h): as exact
-// as fp32 products, at a third of the fp16 rate instead of the sixteenth that fp32 matrix instructions have.  All sums and
-// softmax statistics are fp32 or wider.  e is kept in bf16 for bf16 operands: one rounding of a factor of dz, which is rounded
-// to bf16 for its products anyway; fp32 for fp32.  dz is held in units of a power of two, and without the loss's gradient where
-// that is one number for all rows: (p - 1) at a label is then near -1, which bf16 holds well, instead of the same rounding error in every row; and at the
-// label it comes from expm1(z_label - lse), not from a rounded p.
+// as fp32 products for values from 2^-16 of their tensor's largest on (smaller ones are held to 2^-40 of it), at a third of the
+// fp16 rate instead of the sixteenth that fp32 matrix instructions have.  All sums and softmax statistics are fp32 or wider.  e is
+// kept in bf16 for bf16 operands: one rounding of a factor of dz, which is rounded to bf16 for its products anyway; fp32 for
+// fp32.  dz is held in units of a power of two, and without the loss's gradient where that is one number for all rows: (p - 1) at
+// a label is then near -1, which bf16 holds well, instead of the same rounding error in every row; and at the label it comes from
+// expm1(z_label - lse), not from a rounded p.
 //
 // Masked classes (b = -infinity or the type's lowest value) get probability zero.  A label outside [0, V) that is not `ignore`
 // makes the row's loss and gradients NaN.  x may hold anything in ignored rows: it is packed as zeros there.
@@ -210,133 +211,133 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_logits_kernel(
     bool primed = false;
     int buffer = 0;
     for (long long t = deal.first; t < deal.end; t += deal.stride) {
-    const bool more = t + deal.stride < deal.end;
-    long long m0, n0, next_m0, next_n0;
-    const typename G::Job job = job_at(t, m0, n0), next = more ? job_at(t + deal.stride, next_m0, next_n0) : job;
-    const long long ct = n0 / XT;
-    f32x16 acc[G::TL][G::TR];
-    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
+        const bool more = t + deal.stride < deal.end;
+        long long m0, n0, next_m0, next_n0;
+        const typename G::Job job = job_at(t, m0, n0), next = more ? job_at(t + deal.stride, next_m0, next_n0) : job;
+        const long long ct = n0 / XT;
+        f32x16 acc[G::TL][G::TR];
+        G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wl = wave / WR, wr = wave % WR;
-    for (int i = tid; i < XT; i += G::THREADS) {
-        const long long n = v0 + n0 + i;
-        sbias[i] = n >= vend ? -__builtin_inff() : !bias ? 0.f : bias_bf16 ? xe_load(static_cast<const __hip_bfloat16*>(bias) + n)
-                                                                            : static_cast<const float*>(bias)[n];
-    }
-    for (int i = tid; i < LN; i += G::THREADS) sbeat[i] = 0u;
-    __syncthreads();
-    const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) : 1.f, iw = PL == 2 ? 1.f / xe_scale(amax[1]) : 1.f;
-    const bool full = v0 + n0 + XT <= vend;
-    const int nw = wr * (XT / WR) + 4 * (lane >> 5);            // first class of this lane's, within the tile
-    int own[G::TL];                                             // the row's label within the tile, or out of it
-    bool any_own = false;
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int wl = wave / WR, wr = wave % WR;
+        for (int i = tid; i < XT; i += G::THREADS) {
+            const long long n = v0 + n0 + i;
+            sbias[i] = n >= vend ? -__builtin_inff() : !bias ? 0.f : bias_bf16 ? xe_load(static_cast<const __hip_bfloat16*>(bias) + n)
+                                                                                : static_cast<const float*>(bias)[n];
+        }
+        for (int i = tid; i < LN; i += G::THREADS) sbeat[i] = 0u;
+        __syncthreads();
+        const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) : 1.f, iw = PL == 2 ? 1.f / xe_scale(amax[1]) : 1.f;
+        const bool full = v0 + n0 + XT <= vend;
+        const int nw = wr * (XT / WR) + 4 * (lane >> 5);            // first class of this lane's, within the tile
+        int own[G::TL];                                             // the row's label within the tile, or out of it
+        bool any_own = false;
 #pragma unroll
-    for (int a = 0; a < G::TL; ++a) {
-        const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
-        const long long l = m0 + ml < M ? labels[m0 + ml] - v0 - n0 : -1;
-        own[a] = l >= 0 && l < XT && v0 + n0 + l < vend ? (int)l : -1;
-        any_own |= own[a] >= 0;
-        float mx = -__builtin_inff();
-#pragma unroll
-        for (int b = 0; b < G::TR; ++b)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 bz = *reinterpret_cast<const f32x4*>(sbias + nw + b * 32 + q * 8);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float z = acc[a][b][q * 4 + i];
-                    if (PL == 2) z = z * ix * iw;
-                    z = full || v0 + n0 + nw + b * 32 + q * 8 + i < vend ? z + bz[i] : -__builtin_inff();
-                    acc[a][b][q * 4 + i] = z;
-                    mx = fmaxf(mx, z);
-                }
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (lane < 32) smax[wr * LN + ml] = mx;
-    }
-    any_own = __any(any_own);
-    if (any_own) {                                              // few tiles hold any label of their rows
-#pragma unroll
-        for (int a = 0; a < G::TL; ++a)
+        for (int a = 0; a < G::TL; ++a) {
+            const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
+            const long long l = m0 + ml < M ? labels[m0 + ml] - v0 - n0 : -1;
+            own[a] = l >= 0 && l < XT && v0 + n0 + l < vend ? (int)l : -1;
+            any_own |= own[a] >= 0;
+            float mx = -__builtin_inff();
 #pragma unroll
             for (int b = 0; b < G::TR; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (nw + b * 32 + (r >> 2) * 8 + (r & 3) == own[a]) slab[wl * (LN / WL) + a * 32 + (lane & 31)] = acc[a][b][r];
-    }
-    __syncthreads();
-    const bool keep = E && ct < e_tiles;
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 bz = *reinterpret_cast<const f32x4*>(sbias + nw + b * 32 + q * 8);
 #pragma unroll
-    for (int a = 0; a < G::TL; ++a) {
-        const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
-        float mx = smax[ml];
+                    for (int i = 0; i < 4; ++i) {
+                        float z = acc[a][b][q * 4 + i];
+                        if (PL == 2) z = z * ix * iw;
+                        z = full || v0 + n0 + nw + b * 32 + q * 8 + i < vend ? z + bz[i] : -__builtin_inff();
+                        acc[a][b][q * 4 + i] = z;
+                        mx = fmaxf(mx, z);
+                    }
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (lane < 32) smax[wr * LN + ml] = mx;
+        }
+        any_own = __any(any_own);
+        if (any_own) {                                              // few tiles hold any label of their rows
 #pragma unroll
-        for (int w = 1; w < WR; ++w) mx = fmaxf(mx, smax[w * LN + ml]);
-        const float shift = mx == -__builtin_inff() ? 0.f : mx;
-        float s = 0.f;
-        if (any_own && own[a] >= 0) {                           // does another class of the tile beat the label's?
-            const float zl = slab[ml];
-            bool beat = false;
+            for (int a = 0; a < G::TL; ++a)
+#pragma unroll
+                for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (nw + b * 32 + (r >> 2) * 8 + (r & 3) == own[a]) slab[wl * (LN / WL) + a * 32 + (lane & 31)] = acc[a][b][r];
+        }
+        __syncthreads();
+        const bool keep = E && ct < e_tiles;
+#pragma unroll
+        for (int a = 0; a < G::TL; ++a) {
+            const int ml = wl * (LN / WL) + a * 32 + (lane & 31);
+            float mx = smax[ml];
+#pragma unroll
+            for (int w = 1; w < WR; ++w) mx = fmaxf(mx, smax[w * LN + ml]);
+            const float shift = mx == -__builtin_inff() ? 0.f : mx;
+            float s = 0.f;
+            if (any_own && own[a] >= 0) {                           // does another class of the tile beat the label's?
+                const float zl = slab[ml];
+                bool beat = false;
+#pragma unroll
+                for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float z = acc[a][b][r];
+                        beat |= z > zl || (z == zl && nw + b * 32 + (r >> 2) * 8 + (r & 3) < own[a]);
+                    }
+                if (beat) sbeat[ml] = 1u;                           // all write the same
+            }
 #pragma unroll
             for (int b = 0; b < G::TR; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const float z = acc[a][b][r];
-                    beat |= z > zl || (z == zl && nw + b * 32 + (r >> 2) * 8 + (r & 3) < own[a]);
+                    const float e = __expf(acc[a][b][r] - shift);
+                    acc[a][b][r] = e;
+                    s += e;
                 }
-            if (beat) sbeat[ml] = 1u;                           // all write the same
-        }
+            s += __shfl_xor(s, 32, 64);
+            if (lane < 32) ssum[wr * LN + ml] = s;
+            if (keep && m0 + ml < M) {
 #pragma unroll
-        for (int b = 0; b < G::TR; ++b)
+                for (int b = 0; b < G::TR; ++b) {
+                    if (PL == 2) {
+                        float* out = static_cast<float*>(E) + (m0 + ml) * lde + e0 + n0 + nw + b * 32;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float e = __expf(acc[a][b][r] - shift);
-                acc[a][b][r] = e;
-                s += e;
-            }
-        s += __shfl_xor(s, 32, 64);
-        if (lane < 32) ssum[wr * LN + ml] = s;
-        if (keep && m0 + ml < M) {
-#pragma unroll
-            for (int b = 0; b < G::TR; ++b) {
-                if (PL == 2) {
-                    float* out = static_cast<float*>(E) + (m0 + ml) * lde + e0 + n0 + nw + b * 32;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<f32x4*>(out + q * 8) =
-                            f32x4{acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
+                        for (int q = 0; q < 4; ++q)
+                            *reinterpret_cast<f32x4*>(out + q * 8) =
+                                f32x4{acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
+                    }
                 }
             }
-        }
-        if (PL == 1 && keep) {
-            short* out = static_cast<short*>(E) + (m0 + ml) * lde + e0 + n0 + wr * (XT / WR) + 8 * (lane >> 5);
+            if (PL == 1 && keep) {
+                short* out = static_cast<short*>(E) + (m0 + ml) * lde + e0 + n0 + wr * (XT / WR) + 8 * (lane >> 5);
 #pragma unroll
-            for (int b = 0; b < G::TR; ++b) hgemm::store_bf16_16(acc[a][b], 1.f, out + b * 32, m0 + ml < M);
-        }
-    }
-    __syncthreads();
-    for (int i = tid; i < LN; i += G::THREADS) {
-        const long long m = m0 + i;
-        if (m >= M) continue;
-        float mx = smax[i], s = ssum[i];
-#pragma unroll
-        for (int w = 1; w < WR; ++w) {
-            mx = fmaxf(mx, smax[w * LN + i]);
-            s += ssum[w * LN + i];
-        }
-        const long long tile = v0 / XT + ct;
-        if (tsum) {
-            tmax[tile * M + m] = mx;
-            tsum[tile * M + m] = s;
-            const long long l = labels[m] - v0 - n0;
-            if (l >= 0 && l < XT && v0 + n0 + l < vend) {
-                zlab[m] = slab[i];
-                beaten[m] = sbeat[i] ? 1.f : 0.f;
+                for (int b = 0; b < G::TR; ++b) hgemm::store_bf16_16(acc[a][b], 1.f, out + b * 32, m0 + ml < M);
             }
         }
-    }
-    __syncthreads();                                            // the tile's statistics have been read
+        __syncthreads();
+        for (int i = tid; i < LN; i += G::THREADS) {
+            const long long m = m0 + i;
+            if (m >= M) continue;
+            float mx = smax[i], s = ssum[i];
+#pragma unroll
+            for (int w = 1; w < WR; ++w) {
+                mx = fmaxf(mx, smax[w * LN + i]);
+                s += ssum[w * LN + i];
+            }
+            const long long tile = v0 / XT + ct;
+            if (tsum) {
+                tmax[tile * M + m] = mx;
+                tsum[tile * M + m] = s;
+                const long long l = labels[m] - v0 - n0;
+                if (l >= 0 && l < XT && v0 + n0 + l < vend) {
+                    zlab[m] = slab[i];
+                    beaten[m] = sbeat[i] ? 1.f : 0.f;
+                }
+            }
+        }
+        __syncthreads();                                            // the tile's statistics have been read
     }
 }
 
@@ -576,29 +577,29 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_dx_kernel(const short* __rest
     bool primed = false;
     int buffer = 0;
     for (long long t = deal.first; t < deal.end; t += deal.stride) {
-    const bool more = t + deal.stride < deal.end;
-    long long m0, k0, next_m0, next_k0;
-    int split, next_split;
-    const typename G::Job job = job_at(t, m0, k0, split), next = more ? job_at(t + deal.stride, next_m0, next_k0, next_split) : job;
-    f32x16 acc[G::TL][G::TR];
-    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
+        const bool more = t + deal.stride < deal.end;
+        long long m0, k0, next_m0, next_k0;
+        int split, next_split;
+        const typename G::Job job = job_at(t, m0, k0, split), next = more ? job_at(t + deal.stride, next_m0, next_k0, next_split) : job;
+        f32x16 acc[G::TL][G::TR];
+        G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
 #pragma unroll
-    for (int a = 0; a < G::TL; ++a) {
-        const long long m = m0 + wl * (LN / WL) + a * 32 + (lane & 31);
-        if (m >= M) continue;
+        for (int a = 0; a < G::TL; ++a) {
+            const long long m = m0 + wl * (LN / WL) + a * 32 + (lane & 31);
+            if (m >= M) continue;
 #pragma unroll
-        for (int b = 0; b < G::TR; ++b)
+            for (int b = 0; b < G::TR; ++b)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const long long k = k0 + wr * (XT / WR) + b * 32 + q * 8 + 4 * (lane >> 5);
-                if (k >= ldk) continue;
-                float* out = slab + ((long long)split * M + m) * ldk + k;
-                f32x4 v = {acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
-                if (accumulate) v += *reinterpret_cast<const f32x4*>(out);
-                *reinterpret_cast<f32x4*>(out) = v;
-            }
-    }
+                for (int q = 0; q < 4; ++q) {
+                    const long long k = k0 + wr * (XT / WR) + b * 32 + q * 8 + 4 * (lane >> 5);
+                    if (k >= ldk) continue;
+                    float* out = slab + ((long long)split * M + m) * ldk + k;
+                    f32x4 v = {acc[a][b][q * 4], acc[a][b][q * 4 + 1], acc[a][b][q * 4 + 2], acc[a][b][q * 4 + 3]};
+                    if (accumulate) v += *reinterpret_cast<const f32x4*>(out);
+                    *reinterpret_cast<f32x4*>(out) = v;
+                }
+        }
     }
 }
 
@@ -620,9 +621,10 @@ __global__ __launch_bounds__(256) void xe_dx_finish_kernel(const float* __restri
 // ---- dw[:, v0 ...] = x^T dz
 template <int PL, int OUT_BF16, int LN, int WL, int WR>
 __global__ __launch_bounds__(64 * WL * WR) void xe_dw_kernel(const short* __restrict__ X, long long ldx, const short* __restrict__ dz,
-                                                             long long ldz, long long dz_left,
-                                                    long long M, long long K, long long cols, const unsigned* __restrict__ amax,
-                                                    const float* __restrict__ scale, void* __restrict__ DW, long long V, long long v0) {
+                                                             long long ldz, long long dz_left, long long M, long long K,
+                                                             long long cols, const unsigned* __restrict__ amax,
+                                                             const float* __restrict__ scale, void* __restrict__ DW, long long V,
+                                                             long long v0) {
     typedef Gemm<typename HalfOf<PL>::type, PL, LN, XT, WL, WR, true, true, LN == 64 ? 3 : 2> G;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const long long nrow = (K + LN - 1) / LN, ncol = (cols + XT - 1) / XT;
@@ -638,53 +640,53 @@ __global__ __launch_bounds__(64 * WL * WR) void xe_dw_kernel(const short* __rest
     bool primed = false;
     int buffer = 0;
     for (long long t = deal.first; t < deal.end; t += deal.stride) {
-    const bool more = t + deal.stride < deal.end;
-    long long k0, n0, next_k0, next_n0;
-    const typename G::Job job = job_at(t, k0, n0), next = more ? job_at(t + deal.stride, next_k0, next_n0) : job;
-    f32x16 acc[G::TL][G::TR];
-    G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
-    const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) / XE_DZ_SCALE : 1.f;
-    const float g = *scale;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
+        const bool more = t + deal.stride < deal.end;
+        long long k0, n0, next_k0, next_n0;
+        const typename G::Job job = job_at(t, k0, n0), next = more ? job_at(t + deal.stride, next_k0, next_n0) : job;
+        f32x16 acc[G::TL][G::TR];
+        G::run(job, next, more, primed, buffer, (lds_char*)smem, acc);
+        const float ix = PL == 2 ? 1.f / xe_scale(amax[0]) / XE_DZ_SCALE : 1.f;
+        const float g = *scale;
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / WR, wr = wave % WR;
 #pragma unroll
-    for (int a = 0; a < G::TL; ++a) {
-        const long long k = k0 + wl * (LN / WL) + a * 32 + (lane & 31);
-        if (OUT_BF16) {
-            short* out = static_cast<short*>(DW) + k * V + v0;
-            const long long n = n0 + wr * 64 + 8 * (lane >> 5);
+        for (int a = 0; a < G::TL; ++a) {
+            const long long k = k0 + wl * (LN / WL) + a * 32 + (lane & 31);
+            if (OUT_BF16) {
+                short* out = static_cast<short*>(DW) + k * V + v0;
+                const long long n = n0 + wr * 64 + 8 * (lane >> 5);
 #pragma unroll
-            for (int b = 0; b < G::TR; ++b) {
-                if (n0 + wr * 64 + b * 32 + 32 <= cols) {
-                    hgemm::store_bf16_16(acc[a][b], g, out + n + b * 32, k < K);
-                } else if (k < K) {
+                for (int b = 0; b < G::TR; ++b) {
+                    if (n0 + wr * 64 + b * 32 + 32 <= cols) {
+                        hgemm::store_bf16_16(acc[a][b], g, out + n + b * 32, k < K);
+                    } else if (k < K) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const long long c = n0 + wr * 64 + b * 32 + (r >> 2) * 8 + 4 * (lane >> 5) + (r & 3);
-                        if (c < cols) out[c] = xe_bf16(acc[a][b][r] * g);
+                        for (int r = 0; r < 16; ++r) {
+                            const long long c = n0 + wr * 64 + b * 32 + (r >> 2) * 8 + 4 * (lane >> 5) + (r & 3);
+                            if (c < cols) out[c] = xe_bf16(acc[a][b][r] * g);
+                        }
                     }
                 }
+            } else {
+                float* out = static_cast<float*>(DW) + k * V + v0;
+                if (k >= K) continue;
+#pragma unroll
+                for (int b = 0; b < G::TR; ++b)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const long long c = n0 + wr * 64 + b * 32 + q * 8 + 4 * (lane >> 5);
+                        hgemm::f32x4_any v;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] = acc[a][b][q * 4 + i] * ix * g;
+                        if (c + 4 <= cols) {
+                            *reinterpret_cast<hgemm::f32x4_any*>(out + c) = v;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (c + i < cols) out[c + i] = v[i];
+                        }
+                    }
             }
-        } else {
-            float* out = static_cast<float*>(DW) + k * V + v0;
-            if (k >= K) continue;
-#pragma unroll
-            for (int b = 0; b < G::TR; ++b)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const long long c = n0 + wr * 64 + b * 32 + q * 8 + 4 * (lane >> 5);
-                    hgemm::f32x4_any v;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = acc[a][b][q * 4 + i] * ix * g;
-                    if (c + 4 <= cols) {
-                        *reinterpret_cast<hgemm::f32x4_any*>(out + c) = v;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (c + i < cols) out[c + i] = v[i];
-                    }
-                }
         }
-    }
     }
 }
 
@@ -1026,15 +1028,13 @@ int backward(const Plan& p, const Call& c, const State& st, const void* kept, lo
     return 0;
 }
 
+// The largest sizes: 1048560 rows, 1048576 features, 4194304 classes (32-bit offsets within a tile; rows in blocks of 16 as
+// the second grid dimension).
 bool sizes_ok(long long M, long long K, long long V, int type) {
     return M > 0 && K > 0 && V > 0 && (type == 0 || type == 1) && M <= 65535ll * 16 && K <= (1ll << 20) && V <= (1ll << 22);
 }
 
 }  // namespace
-
-// The largest sizes: 1048560 rows, 1048576 features, 4194304 classes (32-bit offsets within a tile; rows in blocks of 16 as
-// the second grid dimension).
-DTF_API int dtf_linear_xent_supported(long long M, long long K, long long V) { return sizes_ok(M, K, V, 0) ? 1 : 0; }
 
 DTF_API long long dtf_linear_xent_fwd_workspace_bytes(const void* W, long long M, long long K, long long V, int type, int bf16) {
     return sizes_ok(M, K, V, type) ? FwdBuffers(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;

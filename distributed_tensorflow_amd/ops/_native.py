@@ -90,7 +90,6 @@ def kernels():
         "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, C.c_double, c_p, c_p, c_p],
         "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p, c_p],
         "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
-        "dtf_linear_xent_supported": [c_ll] * 3,
         "dtf_linear_xent_fwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 3 + [c_ll, c_i] + [c_p] * 3,
         "dtf_linear_xent_bwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 2 + [c_ll, c_i, c_p, c_i] + [c_p] * 5,
         "dtf_im2col": [c_p, c_p] + [c_i] * 12 + [c_p],

@@ -164,7 +164,10 @@ def linear_softmax_cross_entropy(x, w, labels, b=None, ignore_index: int = -1, r
     without the logits in memory: ``x`` [..., K], ``w`` [K, V], ``b`` [V] or None (all float32 or all bfloat16), int64
     ``labels`` [...].  The loss is float32: the mean over the rows whose label is not ``ignore_index`` (0 when there are
     none), their ``"sum"``, or with ``reduction="none"`` every row's own in the shape of ``labels`` (0 in ignored rows).
-    ``bf16=True`` rounds float32 operands to bfloat16 for the products."""
+    ``bf16=True`` rounds float32 operands to bfloat16 for the products; without it they are as exact as float32 down to 2^-16
+    of their tensor's largest value and keep 2^-40 of that below.  Classes may be masked by a ``b`` of -infinity."""
+    if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
+        raise ValueError("labels must be integers, got %s" % labels.dtype)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
     if tuple(labels.shape) != tuple(x.shape[:-1]):

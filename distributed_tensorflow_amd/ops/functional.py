@@ -353,8 +353,9 @@ def _groupnorm_sizes(x, groups, gamma, beta, *others):
     C = int(x.shape[-1])
     if groups < 1 or C < 1 or C % groups:
         raise ValueError("%d channels do not divide into %d groups" % (C, groups))
-    if C > (1 << 20) or x.shape[0] > (1 << 21):
-        raise ValueError("group normalisation takes at most 2097152 samples and 1048576 channels, got %s" % (tuple(x.shape),))
+    if C > (1 << 20) or x.shape[0] > (1 << 21) or groups > (1 << 14):
+        raise ValueError("group normalisation takes at most 2097152 samples, 1048576 channels and 16384 groups, got %s in %d"
+                         % (tuple(x.shape), groups))
     for name, t in (("gamma", gamma), ("beta", beta)):
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (C,) or not t.is_contiguous()
                               or t.device != x.device):
@@ -430,8 +431,8 @@ def groupnorm_backward(x, dy, gamma, beta, groups, stats, act=ACT_NONE, dgamma=N
         with nv.device_guard(x):
             lib, kind = nv.kernels(), _GROUPNORM_TYPES[x.dtype]
             ws = torch.empty(int(lib.dtf_groupnorm_workspace_doubles(B, S, C, kind)), dtype=torch.float64, device=x.device)
-            rc = lib.dtf_groupnorm_bwd(nv.ptr(x), nv.ptr(dy), nv.ptr(dx), B, S, C, groups, kind, nv.ptr(gamma), nv.ptr(beta), int(act), nv.ptr(stats), nv.ptr(dgamma), nv.ptr(dbeta),
-                                       nv.ptr(ws), nv.stream_ptr())
+            rc = lib.dtf_groupnorm_bwd(nv.ptr(x), nv.ptr(dy), nv.ptr(dx), B, S, C, groups, kind, nv.ptr(gamma), nv.ptr(beta),
+                                       int(act), nv.ptr(stats), nv.ptr(dgamma), nv.ptr(dbeta), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_groupnorm_bwd")
         return dx
     xhat = _groupnorm_xhat(x, groups, stats)
@@ -631,7 +632,8 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False
 
     Rows with the label ``ignore_index`` count for nothing, whatever x holds there; any other label outside ``[0, V)`` makes
     its row's loss NaN.  Classes may be masked by a ``b`` of -infinity (their columns of w must be finite).  ``bf16=True``:
-    float32 operands are rounded to bfloat16 for the products.
+    float32 operands are rounded to bfloat16 for the products; without it each of them, and the logits' gradient, is held to
+    2^-22 of a value or 2^-40 of its tensor's largest value, whichever is more.
 
     Returns ``(loss, state)``: the mean loss of the counted rows (0 without any) or their ``"sum"``, a float32 scalar, or with
     ``reduction="none"`` every row's [M]; the state is what ``linear_xent_backward`` needs.  ``keep=True`` (a backward pass

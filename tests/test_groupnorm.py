@@ -181,6 +181,8 @@ def test_refusals():
         A.group_norm(x, gamma, beta, 3)
     with pytest.raises(ValueError, match="do not divide"):
         A.group_norm(x, gamma, beta, 0)
+    with pytest.raises(ValueError, match="16384 groups"):
+        A.group_norm(torch.zeros(1, 2, 20000), None, None, 20000)
     with pytest.raises(ValueError, match="unsupported activation"):
         A.group_norm(x, gamma, beta, 2, activation="gelu")
     with pytest.raises(ValueError, match="gamma must"):

@@ -113,6 +113,25 @@ def test_loss_and_gradients_of_larger_sizes(gpu_device, dtype, size):
     _check(*_inputs(*size, dtype, "cuda", bias=size[1] != 72), reduction=["mean", "none"][size[2] % 2])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tiles", [0, 1, 3])
+@pytest.mark.parametrize("size", [(100, 72, 1500), (300, 130, 1290)])
+def test_exponentials_that_were_not_kept_are_computed_again(gpu_device, monkeypatch, dtype, tiles, size):
+    x, w, b, labels = _inputs(*size, dtype, "cuda")
+    monkeypatch.setattr(F, "LINEAR_XENT_KEEP_BYTES", tiles * 256 * size[0] * torch.finfo(dtype).bits // 8)
+    state = F.linear_xent_forward(x, w, b, labels, keep=True)[1]
+    assert (state.kept is None) if tiles == 0 else tuple(state.kept.shape) == (size[0], 256 * tiles)
+    _check(x, w, b, labels)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_vocabulary_in_several_pieces(gpu_device, dtype):
+    # dz of more than 512 MB; in float32 the exponentials exceed the budget besides
+    _check(*_inputs(9000, 40, 33001, dtype, "cuda"))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("size", [(65, 129, 255), (5, 64, 1000)])
 def test_rounded_operands(device, size):
@@ -253,6 +272,8 @@ def test_refusals():
         F.linear_xent_backward(x, w, None, labels, state, torch.ones(()), db=torch.empty(20))
     with pytest.raises(ValueError, match="reduction"):
         A.linear_softmax_cross_entropy(x, w, labels, b, reduction="average")
+    with pytest.raises(ValueError, match="integers"):
+        A.linear_softmax_cross_entropy(x, w, labels.float(), b)
     with pytest.raises(ValueError, match="do not fit"):
         A.linear_softmax_cross_entropy(x, w, labels[:3], b)
 
