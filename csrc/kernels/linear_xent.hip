@@ -8,7 +8,9 @@
 //
 // Backward, a piece of the vocabulary at a time: e = exp(z - tile maximum) of the piece -> dz of the piece -> its part of dx
 // (added up in fp32 over pieces and splits) and its columns of dw, whole.  Where the forward pass was told to, it has kept e
-// for the first `kept` classes (as many as fit the caller's memory budget); the logits of the others are computed again.
+// for the first `kept` classes (as many as fit the caller's memory budget); the logits of the others are computed again.  What
+// the forward pass had to pack of x and w (other types than the products', odd strides) stays for the backward pass too if the
+// budget has room (2048 x 1024 x 50021 bf16: @P@).
 // With everything kept a training step is the three products that it cannot do without.
 //
 // Numbers.  bf16 operands multiply as they are.  fp32 operands are scaled by a power of two for each tensor (largest value
@@ -21,7 +23,8 @@
 // expm1(z_label - lse), not from a rounded p.
 //
 // Masked classes (b = -infinity or the type's lowest value) get probability zero.  A label outside [0, V) that is not `ignore`
-// makes the row's loss and gradients NaN.  x may hold anything in ignored rows: it is packed as zeros there.
+// makes the row's loss and gradients NaN.  x may hold anything in ignored rows: it is packed as zeros there, or read in place
+// where only the loss is asked for.
 #include "common.h"
 #include "half_gemm.h"
 
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(256) void xe_dz_kernel(const void* __restrict__ E, 
         const float g = m < M ? rowg[m] : 0.f;
         const float mx = m < M ? tmax[(v0 / XT + blockIdx.x) * M + m] : 0.f;
         const float l = m < M ? lse[m] : 0.f;
-        f[threadIdx.x] = m < M ? g * __expf(mx == -__builtin_inff() ? -__builtin_inff() : mx - l) : 0.f;
+        f[threadIdx.x] = g != 0.f ? g * __expf(mx == -__builtin_inff() ? -__builtin_inff() : mx - l) : 0.f;
         const long long lab = m < M ? labels[m] - v0 - n0 : -1;
         own[threadIdx.x] = lab >= 0 && lab < XT ? (int)lab : -1;
         at_label[threadIdx.x] = own[threadIdx.x] >= 0 && g != 0.f ? g * expm1f(zlab[m] - l) : 0.f;
@@ -723,14 +726,14 @@ Plan make_plan(const void* W, long long M, long long K, long long V, int type, i
     p.piece = lowest(piece, p.tiles * XT);
     p.ldw = p.packs ? p.piece * p.pl : V;
     // dx has few output tiles for its long reduction, which is split: into as many parts as take the least time by the rounds of
-    // 256 workgroups that they need (1.3 us a stage) and the traffic of their sums (4.6 TB/s); eight stages at least a part.
+    // 256 workgroups that they need (a stage takes 1.3 us with 64 rows, 2 us with 256) and the traffic of their sums (4.6 TB/s); eight stages at least a part.
     // (2048 rows, 1024 features: 32 tiles -> 8 parts.)
     const long long out = ((M + (p.small ? 63 : 255)) / (p.small ? 64 : 256)) * ((K + XT - 1) / XT);
     const long long blocks = p.piece / cb;
     double best = 0.0;
     p.splits = 1;
     for (int s = 1; s <= 64 && s * 8 <= (blocks < 8 ? 8 : blocks); ++s) {
-        const double t = (double)((out * s + 255) / 256) / s * (double)blocks * 1.3e-6 + (double)s * M * K * 8 / 4.6e12;
+        const double t = (double)((out * s + 255) / 256) / s * (double)blocks * (p.small ? 1.3e-6 : 2e-6) + (double)s * M * K * 8 / 4.6e12;
         if (s == 1 || t < best) {
             best = t;
             p.splits = s;
@@ -749,6 +752,18 @@ struct Carver {
         T* r = reinterpret_cast<T*>(base + used);
         used += up(n * (long long)sizeof(T), 256);
         return r;
+    }
+};
+
+// The packed operands, where the backward pass takes them over: x, and w if its packed classes are one piece.
+struct Packed {
+    short *x, *w;
+    long long bytes;
+    Packed(const Plan& p, void* base) {
+        Carver c(base);
+        x = c.take<short>(p.M * p.ldx);
+        w = p.packs && p.piece >= p.V ? c.take<short>(p.K * p.ldw) : nullptr;
+        bytes = c.used;
     }
 };
 
@@ -917,9 +932,14 @@ int launch_dw(const Plan& p, const short* x, const short* dz, long long v0, long
     return 0;
 }
 
-int forward(const Plan& p, const Call& c, float* loss, const State& st, void* kept, long long kept_cols, int reduction, float* reduced,
-            void* ws) {
-    const FwdBuffers b(p, ws);
+int forward(const Plan& p, const Call& c, float* loss, const State& st, void* kept, long long kept_cols, void* packed, int reduction,
+            float* reduced, void* ws) {
+    FwdBuffers b(p, ws);
+    if (packed) {
+        const Packed to(p, packed);
+        b.x = to.x;
+        if (to.w) b.w = to.w;
+    }
     float *tmax = st.tmax, *zlab = st.zlab;
     unsigned* amax = st.amax;
     if (p.pl == 2) {
@@ -927,7 +947,10 @@ int forward(const Plan& p, const Call& c, float* loss, const State& st, void* ke
                            c.ignore, static_cast<const float*>(c.W), p.K * p.V, b.partial);
         DTF_CHECK_LAUNCH();
     }
-    XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, b.partial, amax, c.stream));
+    // x in place where the tiles can read it so and no e of an ignored row is kept: such a row's statistics are never looked at
+    const bool direct = p.type == 1 && p.K % 64 == 0 && (reinterpret_cast<uintptr_t>(c.X) & 15) == 0 && !kept && !packed;
+    const short* x = direct ? static_cast<const short*>(c.X) : b.x;
+    if (!direct) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, b.partial, amax, c.stream));
     const long long step = p.packs ? p.piece : p.V;             // where w is read in place the whole vocabulary is one launch
     for (long long v0 = 0; v0 < p.V; v0 += step) {
         const long long cols = lowest(step, p.V - v0);
@@ -935,7 +958,7 @@ int forward(const Plan& p, const Call& c, float* loss, const State& st, void* ke
         long long left;
         XE_TRY(piece_of_w(p, c.W, v0, cols, b.w, amax, c.stream, &w, &left));
         const long long e_tiles = kept_cols > v0 ? (kept_cols - v0) / XT : 0;
-        XE_TRY(logits(p, c, b.x, w, left, v0, v0 + cols, amax, tmax, b.tsum, zlab, b.beaten, kept, kept_cols, v0, e_tiles));
+        XE_TRY(logits(p, c, x, w, left, v0, v0 + cols, amax, tmax, b.tsum, zlab, b.beaten, kept, kept_cols, v0, e_tiles));
     }
     int rows = 16;
     while (rows > 1 && rows / 2 >= p.M) rows /= 2;
@@ -950,15 +973,21 @@ int forward(const Plan& p, const Call& c, float* loss, const State& st, void* ke
     return 0;
 }
 
-int backward(const Plan& p, const Call& c, const State& st, const void* kept, long long kept_cols, int mean, const float* dloss, int stride,
-             void* DX, void* DW, void* DB, void* ws) {
-    const BwdBuffers b(p, ws);
+int backward(const Plan& p, const Call& c, const State& st, const void* kept, long long kept_cols, void* packed, int mean,
+             const float* dloss, int stride, void* DX, void* DW, void* DB, void* ws) {
+    BwdBuffers b(p, ws);
+    bool have_w = false;
+    if (packed) {
+        const Packed from(p, packed);
+        b.x = from.x;
+        if (from.w) b.w = from.w, have_w = true;
+    }
     float *tmax = st.tmax, *zlab = st.zlab, *lse = st.lse, *totals = st.totals;
     unsigned* amax = st.amax;
     hipLaunchKernelGGL(xe_weights_kernel, dim3(1), dim3(1024), 0, c.stream, dloss, stride, totals, mean, c.labels, p.M, p.V, c.ignore,
                        lse, zlab, b.rowg, b.scale);
     DTF_CHECK_LAUNCH();
-    if (DW || kept_cols < p.V) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, nullptr, amax, c.stream));
+    if (!packed && (DW || kept_cols < p.V)) XE_TRY(pack(p, c.X, p.K, p.M, p.K, b.x, p.ldx, c.labels, c.ignore, nullptr, amax, c.stream));
     const int dz_rows = (p.M + 63) / 64 * ((p.piece + XT - 1) / XT) < 1024 ? 16 : 64;
     const long long rowblocks = (p.M + dz_rows - 1) / dz_rows;
     for (long long v0 = 0; v0 < p.V; v0 += p.piece) {
@@ -966,7 +995,10 @@ int backward(const Plan& p, const Call& c, const State& st, const void* kept, lo
         const short* w = nullptr;
         long long left = 0;
         const long long have = kept_cols > v0 ? lowest((kept_cols - v0) / XT, ct) : 0;      // the piece's tiles whose e was kept
-        if (DX || have < ct) XE_TRY(piece_of_w(p, c.W, v0, cols, b.w, amax, c.stream, &w, &left));
+        if (have_w)
+            w = b.w, left = p.K * p.ldw * 2;
+        else if (DX || have < ct)
+            XE_TRY(piece_of_w(p, c.W, v0, cols, b.w, amax, c.stream, &w, &left));
         float* dbp = DB ? b.dbp : nullptr;
         for (int part = 0; part < 2; ++part) {
             const long long t0 = part ? have : 0, t1 = part ? ct : have, at = v0 + t0 * XT;
@@ -1043,29 +1075,36 @@ DTF_API long long dtf_linear_xent_bwd_workspace_bytes(const void* W, long long M
     return sizes_ok(M, K, V, type) ? BwdBuffers(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;
 }
 
+// bytes of the packed operands that a forward call may leave for the backward call
+DTF_API long long dtf_linear_xent_packed_bytes(const void* W, long long M, long long K, long long V, int type, int bf16) {
+    return sizes_ok(M, K, V, type) ? Packed(make_plan(W, M, K, V, type, bf16), nullptr).bytes : -1;
+}
+
 // floats of the state between the two passes
 DTF_API long long dtf_linear_xent_state_floats(long long M, long long V) { return 2 * M + 6 + (V + XT - 1) / XT * M; }
 
 // type: 0 fp32, 1 bf16 (x, w, b alike; b may be null).  bf16 != 0: fp32 operands rounded to bf16 for the products.
 // loss: M floats.  state: [2 M, 2 M + 4) holds the sum of the losses, the rows whose label has the largest logit, the counted
 // rows and the mean, if reduction is not 0; reduced (may be null): the mean (reduction 1) or the sum (2).  kept (may be null):
-// [M, kept_cols] fp32 - bf16 where the products take bf16 -, kept_cols a multiple of 256.
+// [M, kept_cols] fp32 - bf16 where the products take bf16 -, kept_cols a multiple of 256.  packed (may be null): as above.
 DTF_API int dtf_linear_xent_fwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
                                 long long V, int type, int bf16, long long ignore, float* loss, float* state, void* kept,
-                                long long kept_cols, int reduction, float* reduced, void* workspace, hipStream_t stream) {
+                                long long kept_cols, void* packed, int reduction, float* reduced, void* workspace,
+                                hipStream_t stream) {
     if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
     const Call c = {X, W, B, labels, ignore, stream};
-    return forward(make_plan(W, M, K, V, type, bf16), c, loss, State(state, M), kept, kept ? kept_cols : 0, reduction, reduced, workspace);
+    return forward(make_plan(W, M, K, V, type, bf16), c, loss, State(state, M), kept, kept ? kept_cols : 0, packed, reduction, reduced,
+                   workspace);
 }
 
 // dloss: the loss's gradient, one float for all rows (stride 0) or one a row (stride 1); mean != 0: divided by the counted
 // rows (the forward pass had a reduction).  DX, DW, DB may each be null.
 DTF_API int dtf_linear_xent_bwd(const void* X, const void* W, const void* B, const long long* labels, long long M, long long K,
                                 long long V, int type, int bf16, long long ignore, float* state, const void* kept, long long kept_cols,
-                                int mean, const float* dloss, int dloss_stride, void* DX, void* DW, void* DB, void* workspace,
-                                hipStream_t stream) {
+                                void* packed, int mean, const float* dloss, int dloss_stride, void* DX, void* DW, void* DB,
+                                void* workspace, hipStream_t stream) {
     if (!sizes_ok(M, K, V, type) || kept_cols % XT) return -1;
     const Call c = {X, W, B, labels, ignore, stream};
-    return backward(make_plan(W, M, K, V, type, bf16), c, State(state, M), kept, kept ? kept_cols : 0, mean, dloss, dloss_stride, DX, DW,
-                    DB, workspace);
+    return backward(make_plan(W, M, K, V, type, bf16), c, State(state, M), kept, kept ? kept_cols : 0, packed, mean, dloss,
+                    dloss_stride, DX, DW, DB, workspace);
 }

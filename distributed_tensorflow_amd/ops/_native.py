@@ -90,8 +90,8 @@ def kernels():
         "dtf_global_norm": [c_p, c_p, c_p, c_p, c_i, C.c_double, c_p, c_p, c_p],
         "dtf_groupnorm_fwd": [c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_f, c_i, c_p, c_p, c_p],
         "dtf_groupnorm_bwd": [c_p, c_p, c_p, c_ll, c_ll, c_i, c_i, c_i, c_p, c_p, c_i, c_p, c_p, c_p, c_p, c_p],
-        "dtf_linear_xent_fwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 3 + [c_ll, c_i] + [c_p] * 3,
-        "dtf_linear_xent_bwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 2 + [c_ll, c_i, c_p, c_i] + [c_p] * 5,
+        "dtf_linear_xent_fwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 3 + [c_ll, c_p, c_i] + [c_p] * 3,
+        "dtf_linear_xent_bwd": [c_p] * 4 + [c_ll] * 3 + [c_i, c_i, c_ll] + [c_p] * 2 + [c_ll, c_p, c_i, c_p, c_i] + [c_p] * 5,
         "dtf_im2col": [c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_col2im": [c_p, c_p, c_p] + [c_i] * 12 + [c_p],
         "dtf_avgpool_fwd": [c_p, c_p] + [c_i] * 12 + [c_p],
@@ -126,6 +126,7 @@ def kernels():
             fn.restype = c_i
     for name, argtypes in {"dtf_groupnorm_workspace_doubles": [c_ll, c_ll, c_i, c_i],
                            "dtf_linear_xent_state_floats": [c_ll, c_ll],
+                           "dtf_linear_xent_packed_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i],
                            "dtf_linear_xent_fwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i],
                            "dtf_linear_xent_bwd_workspace_bytes": [c_p, c_ll, c_ll, c_ll, c_i, c_i]}.items():
         declare(lib, name, argtypes, c_ll)

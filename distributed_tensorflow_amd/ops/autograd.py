@@ -141,7 +141,7 @@ class _LinearXentFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, labels, ignore_index, reduction, bf16):
         loss, state = F.linear_xent_forward(x, w, b, labels, ignore_index, bf16, True, reduction)
-        ctx.save_for_backward(x, w, b, labels, state.block, state.kept)
+        ctx.save_for_backward(x, w, b, labels, *state[:3])
         ctx.cfg = (ignore_index, reduction, bf16)
         return loss
 

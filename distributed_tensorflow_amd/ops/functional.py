@@ -582,10 +582,11 @@ def softmax_xent(z, labels, grad_out=None, grad_scale=None, stats=None):
 # --------------------------------------------------------------------------- softmax cross-entropy over a large vocabulary
 _XENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 #: what ``linear_xent_forward`` leaves for ``linear_xent_backward``: every row's logsumexp, its label's logit, the totals and
-#: what else the kernels need, in one block of floats; the exponentials of the first logits, or None; the reduction
-LinearXentState = collections.namedtuple("LinearXentState", ["block", "kept", "reduction"])
+#: what else the kernels need, in one block of floats; the exponentials of the first logits, or None; x and w as the products
+#: take them, or None; the reduction
+LinearXentState = collections.namedtuple("LinearXentState", ["block", "kept", "packed", "reduction"])
 _XENT_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
-#: bytes of exponentials that a forward pass with ``keep=True`` may leave for its backward pass (1/288 of an MI355X's memory)
+#: bytes of exponentials and packed operands that a forward pass with ``keep=True`` may leave for its backward pass (1/288 of an MI355X's memory)
 LINEAR_XENT_KEEP_BYTES = 1 << 30
 _XENT_TILE = 256
 
@@ -638,7 +639,8 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False
     Returns ``(loss, state)``: the mean loss of the counted rows (0 without any) or their ``"sum"``, a float32 scalar, or with
     ``reduction="none"`` every row's [M]; the state is what ``linear_xent_backward`` needs.  ``keep=True`` (a backward pass
     will follow): up to ``LINEAR_XENT_KEEP_BYTES`` of the first classes' exponentials stay in the state, which saves the
-    backward pass their part of the product; it computes the others again, piece by piece."""
+    backward pass their part of the product (it computes the others again, piece by piece), and if there is room left the
+    operands that had to be packed."""
     _linear_xent_check(x, w, b, labels)
     if reduction not in _XENT_REDUCTIONS:
         raise ValueError("reduction must be 'mean', 'sum' or 'none', got %r" % (reduction,))
@@ -648,20 +650,23 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False
     if M and x.is_cuda:
         with nv.device_guard(x):
             lib, t, bf16 = nv.kernels(), _XENT_TYPES[x.dtype], int(bool(bf16))
-            cols, kept = 0, None
+            cols, kept, packed = 0, None, None
             if keep:
                 size = 2 if bf16 or t == 1 else 4
                 cols = min(-(-V // _XENT_TILE), LINEAR_XENT_KEEP_BYTES // (M * size * _XENT_TILE)) * _XENT_TILE
             if cols:
                 kept = torch.empty((M, cols), dtype=torch.bfloat16 if size == 2 else torch.float32, device=x.device)
+                room = int(lib.dtf_linear_xent_packed_bytes(nv.ptr(w), M, K, V, t, bf16))
+                if M * cols * size + room <= LINEAR_XENT_KEEP_BYTES:
+                    packed = torch.empty(room, dtype=torch.uint8, device=x.device)
             block = torch.empty(int(lib.dtf_linear_xent_state_floats(M, V)), dtype=torch.float32, device=x.device)
             ws = torch.empty(int(lib.dtf_linear_xent_fwd_workspace_bytes(nv.ptr(w), M, K, V, t, bf16)), dtype=torch.uint8,
                              device=x.device)
             rc = lib.dtf_linear_xent_fwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, bf16, int(ignore_index),
-                                         nv.ptr(rows), nv.ptr(block), nv.ptr(kept), cols, _XENT_REDUCTIONS[reduction],
-                                         nv.ptr(reduced), nv.ptr(ws), nv.stream_ptr())
+                                         nv.ptr(rows), nv.ptr(block), nv.ptr(kept), cols, nv.ptr(packed),
+                                         _XENT_REDUCTIONS[reduction], nv.ptr(reduced), nv.ptr(ws), nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_fwd")
-        return rows if reduced is None else reduced, LinearXentState(block, kept, reduction)
+        return rows if reduced is None else reduced, LinearXentState(block, kept, packed, reduction)
     block = torch.zeros(2 * M + 6, dtype=torch.float32, device=x.device)
     if M:
         _, _, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
@@ -676,7 +681,7 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False
         block[2 * M:2 * M + 4] = torch.stack([total, hits.double(), n.double(), total / n.clamp(min=1)]).float()
     if reduced is not None:
         reduced.copy_(block[2 * M + (3 if reduction == "mean" else 0)])
-    return rows if reduced is None else reduced, LinearXentState(block, None, reduction)
+    return rows if reduced is None else reduced, LinearXentState(block, None, None, reduction)
 
 
 def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index=-1, bf16=False, dx=None, dw=None, db=None):
@@ -708,12 +713,16 @@ def linear_xent_backward(x, w, b, labels, state, dloss, mean=False, ignore_index
     if x.is_cuda:
         with nv.device_guard(x):
             lib, t = nv.kernels(), _XENT_TYPES[x.dtype]
+            if state.packed is not None and state.packed.numel() != int(lib.dtf_linear_xent_packed_bytes(
+                    nv.ptr(w), M, K, V, t, int(bool(bf16)))):
+                raise ValueError("state must be what linear_xent_forward returned for the same call")
             ws = torch.empty(int(lib.dtf_linear_xent_bwd_workspace_bytes(nv.ptr(w), M, K, V, t, int(bool(bf16)))),
                              dtype=torch.uint8, device=x.device)
             rc = lib.dtf_linear_xent_bwd(nv.ptr(x), nv.ptr(w), nv.ptr(b), nv.ptr(labels), M, K, V, t, int(bool(bf16)),
                                          int(ignore_index), nv.ptr(state.block), nv.ptr(kept),
-                                         0 if kept is None else kept.shape[1], int(bool(mean)), nv.ptr(dloss),
-                                         int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw), nv.ptr(db), nv.ptr(ws), nv.stream_ptr())
+                                         0 if kept is None else kept.shape[1], nv.ptr(state.packed), int(bool(mean)),
+                                         nv.ptr(dloss), int(dloss.dim() == 1), nv.ptr(dx), nv.ptr(dw), nv.ptr(db), nv.ptr(ws),
+                                         nv.stream_ptr())
         nv.check(rc, "dtf_linear_xent_bwd")
         return
     x32, w32, z, counted = _linear_xent_logits(x, w, b, labels, ignore_index, bf16)
