@@ -14,21 +14,26 @@
 // Everything is bound by memory.  A sample is one stream of S C values, read in vectors of 16 bytes at any alignment; a
 // workgroup takes T vectors a turn, T a multiple of C / gcd(C, vector): then a thread meets the same channels every turn and
 // keeps their constants in registers.
-//   one   samples up to 128 KB (64 KB in 16 bits): a workgroup holds a sample in registers - x is read once and y written once, dy and x once
-//         and dx once backward: the least there is.  The variance is taken about the mean, from the registers.
+//   one   samples up to 128 KB (64 KB in 16 bits): a workgroup holds a sample in registers - x is read once and y written once,
+//         backward dy and x once and dx once: the least there is.  The variance is taken about the mean, from the registers.
 //   many  larger samples: partial sums of every channel over chunks of a sample (about a pivot, the channel's first value; fp32
 //         over 8 turns, then fp64), joined per group; then one elementwise pass.  x is read twice a direction.
 // All sums have an order that the sizes determine; no atomics.
 //
-// Measured (forward / backward, of the bytes that each cannot do without): 16384 x 24 x 24 x 32 fp32 relu 465 us (5.2 TB/s) /
-// 704 us (5.1 TB/s), a large copy reaching 4.6 TB/s; 64 x 64 x 64 x 256 fp32 silu, read twice, 176 / 190 us; 3 x 129 x 131 x 225
-// bf16 silu (four launches a direction of some 10 us each) 46 / 55 us.  16-bit values with silu are bound by instructions
-// (16384 x 12 x 12 x 64: 183 / 375 us, 3.3 / 2.4 TB/s): the exponential is computed in both passes of the backward kernel, since
+// Whole vectors are taken without a test of every value (bf16 partial sums: 56 -> 33 us) where a second copy of the code does not
+// cost more than the tests: not with sixteen vectors a thread, nor in the backward pass over larger samples.
+//
+// Measured (forward / backward, of the bytes that each cannot do without): 16384 x 24 x 24 x 32 fp32 relu 444 us (5.4 TB/s) /
+// 634 us (5.7 TB/s), a large copy reaching 4.6 TB/s; 64 x 64 x 64 x 256 silu, read twice, fp32 170 / 187 us, bf16 83 / 134 us; 3 x
+// 129 x 131 x 225 bf16 silu (four launches a direction) 35 / 54 us.  16-bit values with silu are bound by instructions
+// (16384 x 12 x 12 x 64: 180 / 359 us, 3.4 / 2.5 TB/s): the exponential is computed in both passes of the backward kernel, since
 // du would have to be kept in 32 bits beside x and dy.
 #include "common.h"
 
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -308,14 +313,25 @@ __global__ __launch_bounds__(512) void grp_one_fwd_kernel(const T* __restrict__ 
     float s2[2][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s2[0][e] = s2[1][e] = 0.f;
+    auto about_mean = [&](int k, auto full) {                  // `full`: a whole vector
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (full || (tid < TH && (k * TH + tid) * VEC + e < N)) {
+                const float d = Elem<T>::get(q[k], e) - ln.hi[e];
+                s2[0][e] += d;
+                s2[1][e] += d * d;
+            }
+    };
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int at = (k * TH + tid) * VEC;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            const float d = tid < TH && at + e < N ? Elem<T>::get(q[k], e) - ln.hi[e] : 0.f;
-            s2[0][e] += d;
-            s2[1][e] += d * d;
+        if (NV > 8) {
+            if (k * TH * VEC >= N) break;
+            about_mean(k, std::false_type());
+        } else {
+            if (tid >= TH || at >= N) break;
+            if (at + VEC <= N) about_mean(k, std::true_type());
+            else about_mean(k, std::false_type());
         }
     }
     grp_channels<float, VEC, 2>(s2, TH, P, C, red, chan);
@@ -375,9 +391,7 @@ __global__ __launch_bounds__(512) void grp_one_bwd_kernel(const T* __restrict__ 
         float s[2][VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[0][e] = s[1][e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            if (k * TH * VEC >= N) break;
+        auto sum_du = [&](int k, auto full) {
             float xh[VEC], u[VEC], d[VEC];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -387,13 +401,25 @@ __global__ __launch_bounds__(512) void grp_one_bwd_kernel(const T* __restrict__ 
             }
             grp_slope<VEC>(u, d, act);
             if constexpr (VEC == 4) qd[k] = Elem<T>::pack(d);          // fp32: du takes dy's registers
-            const int live = tid < TH ? N - (k * TH + tid) * VEC : 0;
+            const int live = full ? VEC : tid < TH ? N - (k * TH + tid) * VEC : 0;
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
                 if (e < live) {
                     s[0][e] += d[e];
                     s[1][e] += d[e] * xh[e];
                 }
+        };
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = (k * TH + tid) * VEC;
+            if (NV > 8) {
+                if (k * TH * VEC >= N) break;
+                sum_du(k, std::false_type());
+            } else {
+                if (tid >= TH || at >= N) break;
+                if (at + VEC <= N) sum_du(k, std::true_type());
+                else sum_du(k, std::false_type());
+            }
         }
         grp_channels<float, VEC, 2>(s, TH, P, C, red, chan);
         for (int i = tid; i < 2 * C; i += blockDim.x) sum[i] += chan[i];
@@ -464,9 +490,10 @@ struct Stream {
 // slab [sample][chunk][2][C] doubles.  Forward: sums of x - pivot and of its square, pivot = the channel's first value of the
 // sample.  Backward: sums of du and du xhat.
 template <typename T, int VEC, bool BWD>
-__global__ __launch_bounds__(512) void grp_partial_kernel(const T* __restrict__ X, const T* __restrict__ DY, long long S, int C, int G, int TH, int P,
-                                   long long chunks, long long per, const float* __restrict__ gamma, const float* __restrict__ beta, int act,
-                                   const float* __restrict__ stats, long long BG, double* __restrict__ slab) {
+__global__ __launch_bounds__(512) void grp_partial_kernel(const T* __restrict__ X, const T* __restrict__ DY, long long S, int C, int G,
+                                                          int TH, int P, long long chunks, long long per,
+                                                          const float* __restrict__ gamma, const float* __restrict__ beta, int act,
+                                                          const float* __restrict__ stats, long long BG, double* __restrict__ slab) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const Stream<VEC> st(S, C, TH, chunks, per);
     const long long b = st.sample;
@@ -487,52 +514,57 @@ __global__ __launch_bounds__(512) void grp_partial_kernel(const T* __restrict__ 
 #pragma unroll
     for (int e = 0; e < VEC; ++e) d[0][e] = d[1][e] = 0.0;
     constexpr int TURNS = BWD ? 4 : 8;
+    // TURNS turns from turn i on; `full`: all of them exist and are whole vectors
+    auto take = [&](long long i, auto full) {
+        u32x4 qx[TURNS], qd[TURNS];
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const long long at = st.at(i + k);
+            const int live = full ? VEC : i + k < st.turn1 ? st.live(at) : 0;
+            qx[k] = live ? grp_load<T, VEC>(x + at, live) : u32x4{0u, 0u, 0u, 0u};
+            if (BWD) qd[k] = live ? grp_load<T, VEC>(dy + at, live) : u32x4{0u, 0u, 0u, 0u};
+        }
+        float s0[VEC], s1[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s0[e] = s1[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < TURNS; ++k) {
+            const int live = full ? VEC : i + k < st.turn1 ? st.live(st.at(i + k)) : 0;
+            if (BWD) {
+                float xh[VEC], u[VEC], du[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    xh[e] = ln.xhat(Elem<T>::get(qx[k], e), e);
+                    u[e] = ln.u(xh[e], e);
+                    du[e] = Elem<T>::get(qd[k], e);
+                }
+                grp_slope<VEC>(u, du, act);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (e < live) {
+                        s0[e] += du[e];
+                        s1[e] += du[e] * xh[e];
+                    }
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (e < live) {
+                        const float off = Elem<T>::get(qx[k], e) - pivot[e];
+                        s0[e] += off;
+                        s1[e] += off * off;
+                    }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            d[0][e] += (double)s0[e];
+            d[1][e] += (double)s1[e];
+        }
+    };
     if (on)
         for (long long i = st.turn0; i < st.turn1; i += TURNS) {
-            u32x4 qx[TURNS], qd[TURNS];
-#pragma unroll
-            for (int k = 0; k < TURNS; ++k) {
-                const long long at = st.at(i + k);
-                const int live = i + k < st.turn1 ? st.live(at) : 0;
-                qx[k] = live ? grp_load<T, VEC>(x + at, live) : u32x4{0u, 0u, 0u, 0u};
-                if (BWD) qd[k] = live ? grp_load<T, VEC>(dy + at, live) : u32x4{0u, 0u, 0u, 0u};
-            }
-            float s0[VEC], s1[VEC];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s0[e] = s1[e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < TURNS; ++k) {
-                const int live = i + k < st.turn1 ? st.live(st.at(i + k)) : 0;
-                if (BWD) {
-                    float xh[VEC], u[VEC], du[VEC];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        xh[e] = ln.xhat(Elem<T>::get(qx[k], e), e);
-                        u[e] = ln.u(xh[e], e);
-                        du[e] = Elem<T>::get(qd[k], e);
-                    }
-                    grp_slope<VEC>(u, du, act);
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (e < live) {
-                            s0[e] += du[e];
-                            s1[e] += du[e] * xh[e];
-                        }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (e < live) {
-                            const float off = Elem<T>::get(qx[k], e) - pivot[e];
-                            s0[e] += off;
-                            s1[e] += off * off;
-                        }
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                d[0][e] += (double)s0[e];
-                d[1][e] += (double)s1[e];
-            }
+            if (i + TURNS <= st.turn1 && st.at(i + TURNS - 1) + VEC <= st.N) take(i, std::true_type());
+            else take(i, std::false_type());
         }
     double* out = slab + (long long)blockIdx.x * 2 * C;
     if (gridDim.y > 1) {                                       // the thread's channels are no other's
@@ -623,9 +655,11 @@ __global__ __launch_bounds__(256) void grp_stats_kernel(const double* __restrict
 
 // The elementwise pass.  Backward: the groups' means of d and d xhat from the channels' sums first.
 template <typename T, int VEC, bool BWD>
-__global__ __launch_bounds__(512) void grp_apply_kernel(const T* __restrict__ X, const T* __restrict__ DY, T* __restrict__ OUT, long long S, int C, int G, int TH,
-                                 long long chunks, long long per, const float* __restrict__ gamma, const float* __restrict__ beta, int act,
-                                 const float* __restrict__ stats, long long BG, const double* __restrict__ csum) {
+__global__ __launch_bounds__(512) void grp_apply_kernel(const T* __restrict__ X, const T* __restrict__ DY, T* __restrict__ OUT,
+                                                        long long S, int C, int G, int TH, long long chunks, long long per,
+                                                        const float* __restrict__ gamma, const float* __restrict__ beta, int act,
+                                                        const float* __restrict__ stats, long long BG,
+                                                        const double* __restrict__ csum) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const Stream<VEC> st(S, C, TH, chunks, per);
     const long long b = st.sample;
@@ -652,19 +686,19 @@ __global__ __launch_bounds__(512) void grp_apply_kernel(const T* __restrict__ X,
             a1[e] = m1[g];
         });
     constexpr int TURNS = 4;
-    for (long long i = st.turn0; i < st.turn1; i += TURNS) {
+    auto take = [&](long long i, auto full) {                  // as in the partial sums
         u32x4 qx[TURNS], qd[TURNS];
 #pragma unroll
         for (int k = 0; k < TURNS; ++k) {
             const long long at = st.at(i + k);
-            const int live = i + k < st.turn1 ? st.live(at) : 0;
+            const int live = full ? VEC : i + k < st.turn1 ? st.live(at) : 0;
             qx[k] = live ? grp_load<T, VEC>(x + at, live) : u32x4{0u, 0u, 0u, 0u};
             if (BWD) qd[k] = live ? grp_load<T, VEC>(dy + at, live) : u32x4{0u, 0u, 0u, 0u};
         }
 #pragma unroll
         for (int k = 0; k < TURNS; ++k) {
             const long long at = st.at(i + k);
-            const int live = i + k < st.turn1 ? st.live(at) : 0;
+            const int live = full ? VEC : i + k < st.turn1 ? st.live(at) : 0;
             if (!live) break;
             float xh[VEC], u[VEC], d[VEC];
 #pragma unroll
@@ -683,6 +717,10 @@ __global__ __launch_bounds__(512) void grp_apply_kernel(const T* __restrict__ X,
             }
             grp_store<T, VEC>(OUT + b * st.N + at, u, live);
         }
+    };
+    for (long long i = st.turn0; i < st.turn1; i += TURNS) {
+        if (!BWD && i + TURNS <= st.turn1 && st.at(i + TURNS - 1) + VEC <= st.N) take(i, std::true_type());
+        else take(i, std::false_type());
     }
 }
 
@@ -753,7 +791,9 @@ int grp_one_lds(const Plan& p, int C, int G, bool bwd) {
 
 template <typename F>
 int with_lds(F* kernel, int bytes) {
-    return bytes <= (48 << 10) ? 0 : (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return bytes <= (48 << 10) ? 0
+                               : (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 struct Args {
@@ -826,10 +866,11 @@ int grp_fwd(const Args& a, const void* X, void* Y, float eps, float* stats, doub
     int rc = whole ? partial<T, Elem<T>::VEC, false>(p, a, x, nullptr, nullptr, ws, csum)
                    : partial<T, 1, false>(p, a, x, nullptr, nullptr, ws, csum);
     if (rc) return rc;
-    hipLaunchKernelGGL(grp_stats_kernel<T>, dim3(loop_grid((a.B * a.G + 3) / 4)), dim3(256), 0, a.stream, csum, x, a.S, a.C, a.G, eps, stats,
-                       a.B * a.G);
+    hipLaunchKernelGGL(grp_stats_kernel<T>, dim3(loop_grid((a.B * a.G + 3) / 4)), dim3(256), 0, a.stream, csum, x, a.S, a.C, a.G, eps,
+                       stats, a.B * a.G);
     DTF_CHECK_LAUNCH();
-    return whole ? apply<T, Elem<T>::VEC, false>(p, a, x, nullptr, y, stats, nullptr) : apply<T, 1, false>(p, a, x, nullptr, y, stats, nullptr);
+    return whole ? apply<T, Elem<T>::VEC, false>(p, a, x, nullptr, y, stats, nullptr)
+                 : apply<T, 1, false>(p, a, x, nullptr, y, stats, nullptr);
 }
 
 template <typename T>

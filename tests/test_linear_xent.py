@@ -194,6 +194,34 @@ def test_masked_classes_have_no_probability(device, dtype, mask):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_ignored_class_of_the_vocabulary(device, dtype):
+    # rows labelled 7 count for nothing, and class 7 keeps its share of the others' probability
+    x, w, b, labels = _inputs(70, 64, 300, dtype, device, ignored=0.0)
+    labels[::3] = 7
+    got, want = [], []
+    for lab, ignore, out in ((labels, 7, got), (torch.where(labels == 7, -1, labels), -1, want)):
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+        loss = A.linear_softmax_cross_entropy(leaves[0], leaves[1], lab, leaves[2], ignore_index=ignore)
+        out += [loss.detach(), *torch.autograd.grad(loss, leaves)]
+    assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_other_orders_in_memory(device):
+    # a head that shares the table of an embedding, w = table.t(); features and labels as views with steps
+    x, w, b, labels = _inputs(40, 64, 300, torch.float32, device)
+    table = w.t().contiguous().requires_grad_()
+    wide = torch.stack([x, x], dim=1).transpose(0, 1).requires_grad_()
+    loss = A.linear_softmax_cross_entropy(wide[0], table.t(), torch.stack([labels, labels], dim=1)[:, 0], b)
+    dx, dt = torch.autograd.grad(loss, (wide, table))
+    x, w = x.requires_grad_(), w.requires_grad_()
+    plain = A.linear_softmax_cross_entropy(x, w, labels, b)
+    ex, ew = torch.autograd.grad(plain, (x, w))
+    assert torch.equal(loss, plain) and torch.equal(dx[0], ex) and not dx[1].any() and torch.equal(dt, ew.t())
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_a_label_outside_the_vocabulary_is_seen(device):
     x, w, b, labels = _inputs(8, 16, 40, torch.float32, device, ignored=0.0)
     labels[2], labels[5] = 40, -3
