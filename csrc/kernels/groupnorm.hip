@@ -23,10 +23,10 @@
 // Whole vectors are taken without a test of every value (bf16 partial sums: 56 -> 33 us) where a second copy of the code does not
 // cost more than the tests: not with sixteen vectors a thread, nor in the backward pass over larger samples.
 //
-// Measured (forward / backward, of the bytes that each cannot do without): 16384 x 24 x 24 x 32 fp32 relu 444 us (5.4 TB/s) /
-// 634 us (5.7 TB/s), a large copy reaching 4.6 TB/s; 64 x 64 x 64 x 256 silu, read twice, fp32 170 / 187 us, bf16 83 / 134 us; 3 x
+// Measured (forward / backward, of the bytes that each cannot do without): 16384 x 24 x 24 x 32 fp32 relu 446 us (5.4 TB/s) /
+// 640 us (5.7 TB/s), a large copy reaching 4.6 TB/s; 64 x 64 x 64 x 256 silu, read twice, fp32 170 / 187 us, bf16 83 / 134 us; 3 x
 // 129 x 131 x 225 bf16 silu (four launches a direction) 35 / 54 us.  16-bit values with silu are bound by instructions
-// (16384 x 12 x 12 x 64: 180 / 359 us, 3.4 / 2.5 TB/s): the exponential is computed in both passes of the backward kernel, since
+// (16384 x 12 x 12 x 64: 169 / 357 us, 3.6 / 2.5 TB/s): the exponential is computed in both passes of the backward kernel, since
 // du would have to be kept in 32 bits beside x and dy.
 #include "common.h"
 
@@ -237,12 +237,19 @@ __device__ __forceinline__ void grp_channels(F (&v)[NA][VEC], int T, int P, int 
             for (int e = 0; e < VEC; ++e) red[a * entries + tid * VEC + e] = v[a][e];
     }
     __syncthreads();
-    for (int i = tid; i < NA * C; i += blockDim.x) {
-        const int a = i / C, c = i - a * C;
-        F s = 0;
-#pragma unroll 4
-        for (int k = c; k < entries; k += C) s += red[a * entries + k];
-        chan[i] = s;
+    // Few channels have many entries each: up to 64 lanes share a channel, eight entries at least a lane, and the sum is fp64
+    // (hundreds of fp32 additions of like numbers all round to one side: with 6 channels of 3060 positions the mean was off by 7e-6).
+    int shift = 0;
+    while (shift < 6 && NA * C << (shift + 1) <= (int)blockDim.x && C << (shift + 4) <= entries) ++shift;
+    const int lanes = 1 << shift, lane = tid & (lanes - 1);
+    for (int i = tid >> shift; __any(i < NA * C); i += blockDim.x >> shift) {
+        const int a = NA == 2 && i >= C ? 1 : 0, c = i - a * C;
+        double s = 0.0;
+        if (i < NA * C)
+#pragma unroll 2
+            for (int k = c + lane * C; k < entries; k += C * lanes) s += (double)red[a * entries + k];
+        for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+        if (lane == 0 && i < NA * C) chan[i] = (F)s;
     }
     __syncthreads();
 }

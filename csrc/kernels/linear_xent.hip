@@ -15,7 +15,7 @@
 //
 // Numbers.  bf16 operands multiply as they are.  fp32 operands are scaled by a power of two for each tensor (largest value
 // in [2^14, 2^15)) and split into two fp16 limbs of 22 bits together, multiplied as three limb products (half_gemm.h): as exact
-// as fp32 products for values from 2^-16 of their tensor's largest on (smaller ones are held to 2^-40 of it), at a third of the
+// as fp32 products for values from 2^-16 of their tensor's largest on (smaller ones are held to 2^-39 of it), at a third of the
 // fp16 rate instead of the sixteenth that fp32 matrix instructions have.  All sums and softmax statistics are fp32 or wider.  e is
 // kept in bf16 for bf16 operands: one rounding of a factor of dz, which is rounded to bf16 for its products anyway; fp32 for
 // fp32.  dz is held in units of a power of two, and without the loss's gradient where that is one number for all rows: (p - 1) at

@@ -165,7 +165,7 @@ def linear_softmax_cross_entropy(x, w, labels, b=None, ignore_index: int = -1, r
     ``labels`` [...].  The loss is float32: the mean over the rows whose label is not ``ignore_index`` (0 when there are
     none), their ``"sum"``, or with ``reduction="none"`` every row's own in the shape of ``labels`` (0 in ignored rows).
     ``bf16=True`` rounds float32 operands to bfloat16 for the products; without it they are as exact as float32 down to 2^-16
-    of their tensor's largest value and keep 2^-40 of that below.  Classes may be masked by a ``b`` of -infinity."""
+    of their tensor's largest value and keep 2^-39 of that below.  Classes may be masked by a ``b`` of -infinity."""
     if labels.is_floating_point() or labels.is_complex() or labels.dtype == torch.bool:
         raise ValueError("labels must be integers, got %s" % labels.dtype)
     if reduction not in ("mean", "sum", "none"):

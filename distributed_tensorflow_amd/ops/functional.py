@@ -634,7 +634,7 @@ def linear_xent_forward(x, w, b, labels, ignore_index=-1, bf16=False, keep=False
     Rows with the label ``ignore_index`` count for nothing, whatever x holds there; any other label outside ``[0, V)`` makes
     its row's loss NaN.  Classes may be masked by a ``b`` of -infinity (their columns of w must be finite).  ``bf16=True``:
     float32 operands are rounded to bfloat16 for the products; without it each of them, and the logits' gradient, is held to
-    2^-22 of a value or 2^-40 of its tensor's largest value, whichever is more.
+    2^-22 of a value or 2^-39 of its tensor's largest value, whichever is more.
 
     Returns ``(loss, state)``: the mean loss of the counted rows (0 without any) or their ``"sum"``, a float32 scalar, or with
     ``reduction="none"`` every row's [M]; the state is what ``linear_xent_backward`` needs.  ``keep=True`` (a backward pass

@@ -130,6 +130,20 @@ def test_values_and_gradients_of_larger_sizes(gpu_device, dtype, shape, groups, 
     _check(shape, groups, dtype, "cuda", act)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,groups", [((47, 90, 34, 6), 3), ((9, 2500, 3), 1), ((5, 8100, 1), 1), ((6, 1021, 5), 5), ((3, 400, 2), 2)])
+def test_few_channels_of_many_positions(gpu_device, dtype, shape, groups):
+    # the channels' own means differ by more than their deviations: long sums of like numbers
+    _check(shape, groups, dtype, "cuda", "tanh")
+    x = _inputs(shape, groups, dtype, "cuda", None)[0]
+    stats = F.groupnorm_forward(x, None, None, groups)[1].double()
+    v = x.double().reshape(shape[0], -1, groups, shape[-1] // groups)
+    mean, var = v.mean((1, 3)), v.var((1, 3), unbiased=False)
+    assert bool(((stats[0] + stats[1] - mean).abs() <= 4 * U * (v - mean[:, None, :, None]).abs().amax((1, 3))).all())
+    assert bool(((stats[2] * torch.sqrt(var + 1e-3) - 1).abs() <= 8 * U).all())
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_one_gradient_at_a_time(device):
     x, gamma, beta, dy = _inputs((3, 5, 7, 12), 4, torch.float32, device, "silu")
