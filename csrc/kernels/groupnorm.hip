@@ -15,7 +15,7 @@
 // workgroup takes T vectors a turn, T a multiple of C / gcd(C, vector): then a thread meets the same channels every turn and
 // keeps their constants in registers.
 //   one   samples up to 128 KB (64 KB in 16 bits): a workgroup holds a sample in registers - x is read once and y written once,
-//         backward dy and x once and dx once: the least there is.  The variance is taken about the mean, from the registers.
+//         backward dy and x once and dx once: the least there is.  The variance is taken about the channels' means, from the registers.
 //   many  larger samples: partial sums of every channel over chunks of a sample (about a pivot, the channel's first value; fp32
 //         over 8 turns, then fp64), joined per group; then one elementwise pass.  x is read twice a direction.
 // All sums have an order that the sizes determine; no atomics.
@@ -254,21 +254,23 @@ __device__ __forceinline__ void grp_channels(F (&v)[NA][VEC], int T, int P, int 
     __syncthreads();
 }
 
-// f(g, sum over the group's channels of value(c)) for every group: a thread a group of few channels, a wave a group of many
-template <typename V, typename Fn>
+// f(g, sum over the group's channels of value(c, g)) for every group: a thread a group of few channels, a wave a group of many
+// UNROLL 1 where registers are short: the forward kernel with sixteen vectors a thread takes 128 of them (443 us; 136 halve the
+// workgroups on a compute unit: 635 us).
+template <int UNROLL, typename V, typename Fn>
 __device__ __forceinline__ void grp_groups(int G, int cg, V value, Fn f) {
     if (cg <= 32) {
         for (int g = threadIdx.x; g < G; g += blockDim.x) {
             double s = 0.0;
-#pragma unroll 4
-            for (int k = 0; k < cg; ++k) s += value(g * cg + k);
+#pragma unroll UNROLL
+            for (int k = 0; k < cg; ++k) s += value(g * cg + k, g);
             f(g, s);
         }
     } else {
         const int lane = threadIdx.x & 63;
         for (int g = threadIdx.x >> 6; g < G; g += blockDim.x >> 6) {
             double s = 0.0;
-            for (int k = lane; k < cg; k += 64) s += value(g * cg + k);
+            for (int k = lane; k < cg; k += 64) s += value(g * cg + k, g);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
             if (lane == 0) f(g, s);
@@ -293,7 +295,8 @@ __global__ __launch_bounds__(512) void grp_one_fwd_kernel(const T* __restrict__ 
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* red = reinterpret_cast<float*>(smem);               // [2][blockDim VEC]
     float* chan = red + 2 * blockDim.x * VEC;                  // [2][C]
-    float* st = chan + 2 * C;                                  // [3][G]
+    float* piv = chan + 2 * C;                                 // [C]
+    float* st = piv + C;                                       // [3][G]
     const long long b = blockIdx.x;
     const int tid = threadIdx.x, cg = C / G, c0 = (int)(((long long)tid * VEC) % C);
     const double n = (double)(N / G);
@@ -312,11 +315,13 @@ __global__ __launch_bounds__(512) void grp_one_fwd_kernel(const T* __restrict__ 
 #pragma unroll
         for (int e = 0; e < VEC; ++e) s[0][e] += Elem<T>::get(q[k], e);
     grp_channels<float, VEC, 1>(s, TH, P, C, red, chan);
-    grp_groups(G, cg, [&](int c) { return (double)chan[c]; }, [&](int g, double v) { st[g] = (float)(v / n); });
+    const double rows = (double)(N / C);
+    for (int c = tid; c < C; c += blockDim.x) piv[c] = (float)((double)chan[c] / rows);
+    __syncthreads();
     grp_forget(q);
     Lane<VEC> ln;
-    grp_walk<VEC>(c0, C, cg, [&](int e, int, int g) { ln.hi[e] = st[g]; });
-    // about the rounded mean: what its rounding left, and the squares
+    grp_walk<VEC>(c0, C, cg, [&](int e, int c, int) { ln.hi[e] = piv[c]; });
+    // about the channel's own mean, so that no partial sum is large: what its rounding left, and the squares
     float s2[2][VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) s2[0][e] = s2[1][e] = 0.f;
@@ -342,9 +347,15 @@ __global__ __launch_bounds__(512) void grp_one_fwd_kernel(const T* __restrict__ 
         }
     }
     grp_channels<float, VEC, 2>(s2, TH, P, C, red, chan);
-    grp_groups(G, cg, [&](int c) { return (double)chan[c]; }, [&](int g, double v) { st[G + g] = (float)(v / n); });
-    grp_groups(G, cg, [&](int c) { return (double)chan[C + c]; }, [&](int g, double v) {
-        const double lo = (double)st[G + g], var = v / n - lo * lo;
+    grp_groups<1>(G, cg, [&](int c, int) { return rows * (double)piv[c] + (double)chan[c]; }, [&](int g, double v) {
+        st[g] = (float)(v / n);
+        st[G + g] = (float)(v / n - (double)st[g]);
+    });
+    grp_groups<1>(G, cg, [&](int c, int g) {
+        const double off = (double)piv[c] - (double)st[g] - (double)st[G + g];   // sum (x - mean)^2 from the sums about piv
+        return (double)chan[C + c] + 2.0 * off * (double)chan[c] + rows * off * off;
+    }, [&](int g, double v) {
+        const double var = v / n;
         const float inv = grp_inv(var > 0.0 || var != var ? var : 0.0, eps);
         st[2 * G + g] = inv;
         stats[b * G + g] = st[g];
@@ -434,9 +445,9 @@ __global__ __launch_bounds__(512) void grp_one_bwd_kernel(const T* __restrict__ 
             __syncthreads();
             continue;
         }
-        grp_groups(G, cg, [&](int c) { return (double)(gamma ? gamma[c] : 1.f) * (double)chan[c]; },
+        grp_groups<4>(G, cg, [&](int c, int) { return (double)(gamma ? gamma[c] : 1.f) * (double)chan[c]; },
                    [&](int g, double v) { m0[g] = (float)(v / n); });
-        grp_groups(G, cg, [&](int c) { return (double)(gamma ? gamma[c] : 1.f) * (double)chan[C + c]; },
+        grp_groups<4>(G, cg, [&](int c, int) { return (double)(gamma ? gamma[c] : 1.f) * (double)chan[C + c]; },
                    [&](int g, double v) { m1[g] = (float)(v / n); });
         grp_forget(qx);
         grp_forget(qd);
@@ -678,8 +689,9 @@ __global__ __launch_bounds__(512) void grp_apply_kernel(const T* __restrict__ X,
     if (BWD) {
         const double* s = csum + b * 2 * C;
         const double n = (double)S * (double)cg;
-        grp_groups(G, cg, [&](int c) { return (double)(gamma ? gamma[c] : 1.f) * s[c]; }, [&](int g, double v) { m0[g] = (float)(v / n); });
-        grp_groups(G, cg, [&](int c) { return (double)(gamma ? gamma[c] : 1.f) * s[C + c]; },
+        grp_groups<4>(G, cg, [&](int c, int) { return (double)(gamma ? gamma[c] : 1.f) * s[c]; },
+                      [&](int g, double v) { m0[g] = (float)(v / n); });
+        grp_groups<4>(G, cg, [&](int c, int) { return (double)(gamma ? gamma[c] : 1.f) * s[C + c]; },
                    [&](int g, double v) { m1[g] = (float)(v / n); });
     }
     if ((int)threadIdx.x >= st.live_threads) return;
@@ -793,7 +805,7 @@ unsigned loop_grid(long long items) { return (unsigned)(items < (1 << 20) ? item
 
 template <typename T>
 int grp_one_lds(const Plan& p, int C, int G, bool bwd) {
-    return (2 * p.block * Elem<T>::VEC + 2 * C + (bwd ? 2 * C + 2 * G : 3 * G)) * 4;
+    return (2 * p.block * Elem<T>::VEC + 2 * C + (bwd ? 2 * C + 2 * G : C + 3 * G)) * 4;
 }
 
 template <typename F>
