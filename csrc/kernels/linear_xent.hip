@@ -708,7 +708,7 @@ struct Plan {
     long long M, K, V;
     int type, pl;              // 0 fp32, 1 bf16 operands; limbs a value
     bool packs;                // w has to be packed
-    bool small;                // 64 rows of x a tile
+    bool small, small_dx;      // 64 rows of x a tile: for the logits, for dx
     long long ldx, ldw, piece, tiles;
     long long esize;
     int splits;                // of the classes of a piece for dx
@@ -721,10 +721,13 @@ Plan make_plan(const void* W, long long M, long long K, long long V, int type, i
     p.pl = type == 0 && !bf16 ? 2 : 1;
     const int cb = 64 / p.pl;
     p.packs = type == 0 || V % 8 != 0 || (reinterpret_cast<uintptr_t>(W) & 15) != 0;
-    // 64 rows a tile while they waste less of the matrix instructions than they read w more often
-    p.small = M <= 128;
     p.ldx = up(K, cb) * p.pl;
     p.tiles = (V + XT - 1) / XT;
+    // 64 rows a tile where few rows would leave most of a larger one empty, or where the larger ones do not fill the chip: a stage
+    // takes some 1.3 us with 64 rows, 2 us with 256, a round 256 workgroups.  (346 rows, 2752 features, 1792 classes, fp32, loss
+    // alone: 110 us with 42 tiles, 187 us with 14.)
+    const double few = 1.3e-6, many = 2e-6;
+    p.small = M <= 128 || (double)(((M + 63) / 64 * p.tiles + 255) / 256) * few < (double)(((M + 255) / 256 * p.tiles + 255) / 256) * many;
     p.esize = p.pl == 2 ? 4 : 2;
     long long piece = XE_PIECE_BYTES / (M * 2 * p.pl);
     if (p.packs) piece = lowest(piece, XE_PACK_BYTES / (K * 2 * p.pl));
@@ -732,18 +735,21 @@ Plan make_plan(const void* W, long long M, long long K, long long V, int type, i
     if (piece < XT) piece = XT;
     p.piece = lowest(piece, p.tiles * XT);
     p.ldw = p.packs ? p.piece * p.pl : V;
-    // dx has few output tiles for its long reduction, which is split: into as many parts as take the least time by the rounds of
-    // 256 workgroups that they need (a stage takes 1.3 us with 64 rows, 2 us with 256) and the traffic of their sums (4.6 TB/s);
-    // eight stages at least a part.  (2048 rows, 1024 features: 32 tiles -> 8 parts.)
-    const long long out = ((M + (p.small ? 63 : 255)) / (p.small ? 64 : 256)) * ((K + XT - 1) / XT);
+    // dx has few output tiles for its long reduction, which is split: into as many parts as take the least time by the rounds that
+    // they need and the traffic of their sums (4.6 TB/s), with tiles of either height; eight stages at least a part.
+    // (2048 rows, 1024 features: 32 tiles -> 8 parts.)
     const long long blocks = p.piece / cb;
     double best = 0.0;
-    p.splits = 1;
-    for (int s = 1; s <= 64 && s * 8 <= (blocks < 8 ? 8 : blocks); ++s) {
-        const double t = (double)((out * s + 255) / 256) / s * (double)blocks * (p.small ? 1.3e-6 : 2e-6) + (double)s * M * K * 8 / 4.6e12;
-        if (s == 1 || t < best) {
-            best = t;
-            p.splits = s;
+    p.splits = 0;
+    for (int low = M <= 128 ? 1 : 0; low < 2; ++low) {
+        const long long out = ((M + (low ? 63 : 255)) / (low ? 64 : 256)) * ((K + XT - 1) / XT);
+        for (int n = 1; n <= 64 && n * 8 <= (blocks < 8 ? 8 : blocks); ++n) {
+            const double t = (double)((out * n + 255) / 256) / n * (double)blocks * (low ? few : many) + (double)n * M * K * 8 / 4.6e12;
+            if (p.splits == 0 || t < best) {
+                best = t;
+                p.splits = n;
+                p.small_dx = low != 0;
+            }
         }
     }
     p.ldk = up(K, 4);
@@ -1029,10 +1035,10 @@ int backward(const Plan& p, const Call& c, const State& st, const void* kept, lo
         if (DX) {
             const int first = v0 == 0;
             if (p.pl == 1)
-                XE_TRY(p.small ? (launch_dx<1, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
+                XE_TRY(p.small_dx ? (launch_dx<1, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
                                : (launch_dx<1, 256, 2, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream)));
             else
-                XE_TRY(p.small ? (launch_dx<2, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
+                XE_TRY(p.small_dx ? (launch_dx<2, 64, 1, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream))
                                : (launch_dx<2, 256, 2, 4>(p, b.dz, w, left, cols, first, b.slab, c.stream)));
         }
         if (DW) {
