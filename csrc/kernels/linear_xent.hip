@@ -23,9 +23,9 @@
 // expm1(z_label - lse), not from a rounded p.
 //
 // What bounds it: the three products (half_gemm.h), tiles of 256 x 256 by workgroups that stay and take the next tile's first stage
-// along; tiles of 64 rows up to 128 rows and where the larger ones would not fill the chip, bound by their loads.  Everything else is one pass over what
-// it reads.  Measured, loss and gradients of rows x features x classes: 2048 x 1024 x 50021 bf16 834 us (logits 298, dx 223, dw 276,
-// dz 76 at 5.4 TB/s, packing 41 us), 4096 x 1024 x 32000 fp32 2.30 ms (860, 716, 734, 213 at 4.9 TB/s), 8192 x 2048 x 65536 bf16
+// along; tiles of 64 rows up to 128 rows and where the larger ones would not fill the chip, bound by their loads.  Everything
+// else is one pass over what it reads.  Measured, loss and gradients of rows x features x classes: 2048 x 1024 x 50021 bf16 834 us
+// (logits 298, dx 223, dw 276, dz 76 at 5.4 TB/s, packing 41 us), 4096 x 1024 x 32000 fp32 2.30 ms (860, 716, 734, 213 at 4.9 TB/s), 8192 x 2048 x 65536 bf16
 // 6.37 ms (products at 1.12 PFLOP/s), 128 x 512 x 10001 fp32 101 us in twelve launches; the loss of one row, 512 x 32000 bf16,
 // 18 us in two.
 //
